@@ -226,4 +226,73 @@ hipError_t launch_qk_norm_rope(uint32_t tokens, uint32_t heads, uint32_t head_di
                                int dtype, const void* x, uint32_t x_stride, void* out, uint32_t out_stride,
                                hipStream_t s);
 
+// The 4-bit key / value cache (cache4.hip): shapes, layout and meaning as in we_cache4.h. Strides are in values; lens,
+// counts, ... are device arrays.
+struct Cache4 {
+  uint32_t batch, kv_heads, dim, capacity;
+  uint8_t* kc;   // K codes, K scales, V codes, V scales
+  uint32_t* ks;
+  uint8_t* vc;
+  uint32_t* vs;
+};
+struct Cache4Append {
+  Cache4 c;
+  uint32_t tokens;
+  int dtype;
+  const void* k;
+  const void* v;
+  uint32_t k_stride, v_stride;
+  const int32_t* counts;
+  const int32_t* lens;
+  int32_t* lens_out;
+  const int32_t* seen;
+  int32_t* seen_out;
+  int32_t* pos;
+  float* weight;
+};
+hipError_t cache4_append_launch(const Cache4Append& L, hipStream_t s);
+struct Cache4Load {
+  Cache4 c;
+  uint32_t tokens;
+  int dtype;
+  void* k;
+  void* v;
+  uint32_t k_stride, v_stride;
+  const int32_t* first;
+  const int32_t* lens;
+};
+hipError_t cache4_load_launch(const Cache4Load& L, hipStream_t s);
+struct Cache4Attention {
+  Cache4 c;
+  uint32_t tokens, heads;
+  int causal, dtype;
+  const void* q;
+  uint32_t q_stride;
+  const int32_t* counts;
+  const int32_t* lens;
+  uint32_t max_len;
+  const float* weight;
+  float* weight_out;
+  void* out;
+  uint32_t out_stride;
+  void* scratch;  // cache4_attention_scratch(L) bytes
+};
+size_t cache4_attention_scratch(const Cache4Attention& L);
+hipError_t cache4_attention_launch(const Cache4Attention& L, hipStream_t s);
+struct Cache4Evict {
+  Cache4 c;
+  uint32_t keep, max_len;
+  const int32_t* lens;
+  int32_t* lens_out;
+  const float* weight;
+  float* weight_out;
+  const int32_t* pos;
+  int32_t* pos_out;
+  const int32_t* seen;
+  uint32_t sinks, recent;
+  void* scratch;  // cache4_evict_scratch(L) bytes
+};
+size_t cache4_evict_scratch(const Cache4Evict& L);
+hipError_t cache4_evict_launch(const Cache4Evict& L, hipStream_t s);
+
 }  // namespace we

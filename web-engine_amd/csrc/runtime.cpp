@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/we.h"
+#include "../../include/we_cache4.h"
 #include "internal.h"
 
 namespace {
@@ -1499,6 +1500,210 @@ int we_dequant_int4(we_ctx* ctx, const uint32_t* words, const uint16_t* scales, 
   if (rc) return rc;
   hipError_t e = we::launch_dequant_int4(words, scales, rows, k, group, out, ctx->compute);
   return e == hipSuccess ? WE_OK : hip_fail(ctx, e, "dequant launch");
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------------------------------ 4-bit key / value cache
+
+namespace {
+
+// An operand of a cache call, for the check that what a call writes overlaps nothing else of it.
+struct Operand {
+  const void* p;
+  uint64_t bytes;
+  const char* name;
+  const void* same;  // written operands: the input this may be (its own array); inputs: null
+  bool written;
+};
+
+int check_operands(we_ctx* ctx, const Operand* ops, size_t n) {
+  for (size_t i = 0; i < n; i++)
+    if (ops[i].p) {
+      if (const int rc = check_span(ctx, ops[i].p, ops[i].bytes, ops[i].name)) return rc;
+    }
+  for (size_t i = 0; i < n; i++) {
+    if (!ops[i].p || !ops[i].written) continue;
+    const uintptr_t a = (uintptr_t)ops[i].p;
+    for (size_t j = 0; j < n; j++) {
+      if (j == i || !ops[j].p || (ops[j].written && j < i)) continue;
+      if (!ops[j].written && ops[j].p == ops[i].same) continue;
+      const uintptr_t b = (uintptr_t)ops[j].p;
+      if (a < b + ops[j].bytes && b < a + ops[i].bytes)
+        return fail(ctx, WE_EINVAL, "%s overlaps %s", ops[i].name, ops[j].name);
+    }
+  }
+  return WE_OK;
+}
+
+int cache4_shape(we_ctx* ctx, const we_cache4* c) {
+  if (!c) return fail(ctx, WE_EINVAL, "cache is null");
+  if (c->dim == 0 || c->dim % WE_CACHE4_GROUP || c->dim > 256)
+    return fail(ctx, WE_EUNSUPPORTED, "cache dim must be a multiple of %u and at most 256, got %u", WE_CACHE4_GROUP, c->dim);
+  if (c->capacity == 0 || c->capacity % 64 || c->capacity > (1u << 24))
+    return fail(ctx, WE_EINVAL, "cache capacity must be a multiple of 64 from 64 to %u, got %u", 1u << 24, c->capacity);
+  if (c->batch == 0 || c->batch > 65535 || c->kv_heads == 0 || c->kv_heads > 65535)
+    return fail(ctx, WE_EINVAL, "cache batch and kvHeads must be from 1 to 65535, got %u and %u", c->batch, c->kv_heads);
+  return WE_OK;
+}
+
+uint64_t cache4_slots(const we_cache4* c) { return (uint64_t)c->batch * c->kv_heads * c->capacity; }
+uint64_t cache4_size(const we_cache4* c) { return cache4_slots(c) * (c->dim + c->dim / WE_CACHE4_GROUP * 8); }
+
+// The cache's shape and buffer, checked, with its four regions.
+int cache4_open(we_ctx* ctx, const we_cache4* c, we::Cache4* out) {
+  if (!ctx) return fail(ctx, WE_EINVAL, "context is null");
+  if (const int rc = cache4_shape(ctx, c)) return rc;
+  if (!c->data) return fail(ctx, WE_EINVAL, "cache data is null");
+  if ((uintptr_t)c->data % 16) return fail(ctx, WE_EINVAL, "cache data must be 16-byte aligned");
+  const uint64_t codes = cache4_slots(c) * (c->dim / 2), scales = cache4_slots(c) * (c->dim / WE_CACHE4_GROUP) * 4;
+  uint8_t* p = (uint8_t*)c->data;
+  *out = we::Cache4{c->batch, c->kv_heads, c->dim, c->capacity, p, (uint32_t*)(p + codes), p + codes + scales,
+                    (uint32_t*)(p + 2 * codes + scales)};
+  HIP_OK(ctx, hipSetDevice(ctx->device), "hipSetDevice");
+  return WE_OK;
+}
+
+// Rows of `heads` heads: their stride (0: packed) and the bytes of batch * tokens of them.
+int cache4_rows(we_ctx* ctx, const we_cache4* c, uint32_t tokens, uint32_t heads, int dtype, const void* p, uint32_t stride,
+                const char* name, uint32_t* stride_out, uint64_t* bytes) {
+  const uint64_t row = (uint64_t)heads * c->dim, st = stride ? stride : row;
+  const uint32_t align = dtype == WE_F32 ? 4 : 8;
+  if (st < row) return fail(ctx, WE_EINVAL, "%s stride below the %llu values of its heads", name, (unsigned long long)row);
+  if (st % align || st > 0xffffffffull)
+    return fail(ctx, WE_EINVAL, "%s stride must be a multiple of %u below 2^32, got %llu", name, align, (unsigned long long)st);
+  if ((uintptr_t)p % 16) return fail(ctx, WE_EINVAL, "%s must be 16-byte aligned", name);
+  const uint64_t n = (uint64_t)c->batch * tokens;
+  *stride_out = (uint32_t)st;
+  *bytes = n ? ((n - 1) * st + row) * elem_bytes(dtype) : 0;
+  return WE_OK;
+}
+
+int cache4_tokens(we_ctx* ctx, uint32_t tokens, int dtype, const char* what) {
+  if (!is_act(dtype)) return fail(ctx, WE_EINVAL, "%s dtype %d is not f32 / f16 / bf16", what, dtype);
+  if (tokens > (1u << 24)) return fail(ctx, WE_EINVAL, "%s takes at most %u tokens, got %u", what, 1u << 24, tokens);
+  return WE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int we_cache4_bytes(we_ctx* ctx, const we_cache4* cache, uint64_t* bytes) {
+  if (!bytes) return fail(ctx, WE_EINVAL, "output pointer is null");
+  if (const int rc = cache4_shape(ctx, cache)) return rc;
+  *bytes = cache4_size(cache);
+  return WE_OK;
+}
+
+int we_cache4_append(we_ctx* ctx, const we_cache4* cache, uint32_t tokens, int dtype, const void* k, uint32_t k_stride,
+                     const void* v, uint32_t v_stride, const int32_t* counts, const int32_t* lens, int32_t* lens_out,
+                     const int32_t* seen, int32_t* seen_out, int32_t* pos, float* weight) {
+  we::Cache4Append L{};
+  int rc = cache4_open(ctx, cache, &L.c);
+  if (!rc) rc = cache4_tokens(ctx, tokens, dtype, "cache append");
+  if (rc) return rc;
+  if (!lens || !lens_out) return fail(ctx, WE_EINVAL, "cache lens or lens_out is null");
+  if (seen_out && !seen) return fail(ctx, WE_EINVAL, "seen_out without seen");
+  if (tokens && (!k || !v)) return fail(ctx, WE_EINVAL, "cache append k or v is null");
+  uint64_t kb = 0, vb = 0;
+  rc = cache4_rows(ctx, cache, tokens, cache->kv_heads, dtype, k, k_stride, "k", &L.k_stride, &kb);
+  if (!rc) rc = cache4_rows(ctx, cache, tokens, cache->kv_heads, dtype, v, v_stride, "v", &L.v_stride, &vb);
+  if (rc) return rc;
+  const uint64_t per = (uint64_t)cache->batch * 4, slots = cache4_slots(cache) * 4;
+  const Operand ops[] = {{cache->data, cache4_size(cache), "cache data", nullptr, true}, {lens_out, per, "lens_out", lens, true},
+                         {seen_out, per, "seen_out", seen, true},                        {pos, slots, "pos", nullptr, true},
+                         {weight, slots, "weight", nullptr, true},                       {k, kb, "k", nullptr, false},
+                         {v, vb, "v", nullptr, false},                                   {counts, per, "counts", nullptr, false},
+                         {lens, per, "lens", nullptr, false},                            {seen, per, "seen", nullptr, false}};
+  if ((rc = check_operands(ctx, ops, sizeof ops / sizeof ops[0]))) return rc;
+  L.tokens = tokens, L.dtype = dtype, L.k = k, L.v = v, L.counts = counts, L.lens = lens, L.lens_out = lens_out;
+  L.seen = seen, L.seen_out = seen_out, L.pos = pos, L.weight = weight;
+  const hipError_t e = we::cache4_append_launch(L, ctx->compute);
+  return e == hipSuccess ? WE_OK : hip_fail(ctx, e, "cache append launch");
+}
+
+int we_cache4_load(we_ctx* ctx, const we_cache4* cache, uint32_t tokens, const int32_t* first, const int32_t* lens, int dtype,
+                   void* k, uint32_t k_stride, void* v, uint32_t v_stride) {
+  we::Cache4Load L{};
+  int rc = cache4_open(ctx, cache, &L.c);
+  if (!rc) rc = cache4_tokens(ctx, tokens, dtype, "cache load");
+  if (rc) return rc;
+  if (!lens) return fail(ctx, WE_EINVAL, "cache lens is null");
+  uint64_t kb = 0, vb = 0;
+  rc = cache4_rows(ctx, cache, tokens, cache->kv_heads, dtype, k, k_stride, "k", &L.k_stride, &kb);
+  if (!rc) rc = cache4_rows(ctx, cache, tokens, cache->kv_heads, dtype, v, v_stride, "v", &L.v_stride, &vb);
+  if (rc) return rc;
+  const uint64_t per = (uint64_t)cache->batch * 4;
+  const Operand ops[] = {{k, kb, "k", nullptr, true},
+                         {v, vb, "v", nullptr, true},
+                         {cache->data, cache4_size(cache), "cache data", nullptr, false},
+                         {first, per, "first", nullptr, false},
+                         {lens, per, "lens", nullptr, false}};
+  if ((rc = check_operands(ctx, ops, sizeof ops / sizeof ops[0]))) return rc;
+  L.tokens = tokens, L.dtype = dtype, L.k = k, L.v = v, L.first = first, L.lens = lens;
+  const hipError_t e = we::cache4_load_launch(L, ctx->compute);
+  return e == hipSuccess ? WE_OK : hip_fail(ctx, e, "cache load launch");
+}
+
+int we_cache4_attention(we_ctx* ctx, const we_cache4* cache, uint32_t tokens, uint32_t heads, int causal, int dtype,
+                        const void* q, uint32_t q_stride, const int32_t* counts, const int32_t* lens, uint32_t max_len,
+                        const float* weight, float* weight_out, void* out, uint32_t out_stride) {
+  we::Cache4Attention L{};
+  int rc = cache4_open(ctx, cache, &L.c);
+  if (!rc) rc = cache4_tokens(ctx, tokens, dtype, "cache attention");
+  if (rc) return rc;
+  if (heads == 0 || heads % cache->kv_heads) return fail(ctx, WE_EINVAL, "heads must be a multiple of kvHeads");
+  if ((uint64_t)tokens * heads > 0x7fffffffull)
+    return fail(ctx, WE_EINVAL, "cache attention takes fewer than 2^31 query heads of a sequence");
+  if (!lens) return fail(ctx, WE_EINVAL, "cache lens is null");
+  if (weight && !weight_out) return fail(ctx, WE_EINVAL, "weight without weight_out");
+  if (tokens && (!q || !out)) return fail(ctx, WE_EINVAL, "cache attention q or out is null");
+  uint64_t qb = 0, ob = 0;
+  rc = cache4_rows(ctx, cache, tokens, heads, dtype, q, q_stride, "q", &L.q_stride, &qb);
+  if (!rc) rc = cache4_rows(ctx, cache, tokens, heads, dtype, out, out_stride, "out", &L.out_stride, &ob);
+  if (rc) return rc;
+  const uint64_t per = (uint64_t)cache->batch * 4, slots = cache4_slots(cache) * 4;
+  const Operand ops[] = {{out, ob, "out", nullptr, true},        {weight_out, slots, "weight_out", weight, true},
+                         {q, qb, "q", nullptr, false},           {cache->data, cache4_size(cache), "cache data", nullptr, false},
+                         {counts, per, "counts", nullptr, false}, {lens, per, "lens", nullptr, false},
+                         {weight, slots, "weight", nullptr, false}};
+  if ((rc = check_operands(ctx, ops, sizeof ops / sizeof ops[0]))) return rc;
+  L.tokens = tokens, L.heads = heads, L.causal = causal ? 1 : 0, L.dtype = dtype, L.q = q, L.counts = counts, L.lens = lens;
+  L.max_len = max_len && max_len < cache->capacity ? max_len : cache->capacity;
+  L.weight = weight, L.weight_out = weight_out, L.out = out;
+  if (const size_t need = we::cache4_attention_scratch(L)) {
+    if ((rc = ensure_scratch(ctx, need))) return rc;
+    L.scratch = ctx->scratch;
+  }
+  const hipError_t e = we::cache4_attention_launch(L, ctx->compute);
+  return e == hipSuccess ? WE_OK : hip_fail(ctx, e, "cache attention launch");
+}
+
+int we_cache4_evict(we_ctx* ctx, const we_cache4* cache, uint32_t keep, const int32_t* lens, int32_t* lens_out,
+                    uint32_t max_len, const float* weight, float* weight_out, const int32_t* pos, int32_t* pos_out,
+                    const int32_t* seen, uint32_t sinks, uint32_t recent) {
+  we::Cache4Evict L{};
+  int rc = cache4_open(ctx, cache, &L.c);
+  if (rc) return rc;
+  if (!lens || !lens_out || !weight || !weight_out || !pos || !pos_out)
+    return fail(ctx, WE_EINVAL, "cache evict needs lens, weight and pos and their outputs");
+  if (sinks > 0x7fffffffu || recent > 0x7fffffffu) return fail(ctx, WE_EINVAL, "sinks and recent must be below 2^31");
+  const uint64_t per = (uint64_t)cache->batch * 4, slots = cache4_slots(cache) * 4;
+  const Operand ops[] = {{cache->data, cache4_size(cache), "cache data", nullptr, true}, {lens_out, per, "lens_out", lens, true},
+                         {weight_out, slots, "weight_out", weight, true},                {pos_out, slots, "pos_out", pos, true},
+                         {lens, per, "lens", nullptr, false},                            {weight, slots, "weight", nullptr, false},
+                         {pos, slots, "pos", nullptr, false},                            {seen, per, "seen", nullptr, false}};
+  if ((rc = check_operands(ctx, ops, sizeof ops / sizeof ops[0]))) return rc;
+  L.keep = keep, L.lens = lens, L.lens_out = lens_out, L.weight = weight, L.weight_out = weight_out, L.pos = pos;
+  L.pos_out = pos_out, L.seen = seen ? seen : lens, L.sinks = sinks, L.recent = recent;
+  L.max_len = max_len && max_len < cache->capacity ? max_len : cache->capacity;
+  if (const size_t need = we::cache4_evict_scratch(L)) {
+    if ((rc = ensure_scratch(ctx, need))) return rc;
+    L.scratch = ctx->scratch;
+  }
+  const hipError_t e = we::cache4_evict_launch(L, ctx->compute);
+  return e == hipSuccess ? WE_OK : hip_fail(ctx, e, "cache evict launch");
 }
 
 }  // extern "C"

@@ -1,4 +1,4 @@
-"""Python host side of the MI355X matmul path: a ctypes binding of libwe.so (include/we.h) and a
+"""Python host side of the MI355X matmul path: a ctypes binding of libwe.so (include/we.h, we_cache4.h) and a
 mirror of the reference's operator API over it.
 
   Graph                 src/gpu/graph.ts:26-155   (buffer / read / free / mark / release / copy / destroy / stats)
@@ -10,6 +10,7 @@ mirror of the reference's operator API over it.
   swiglu, sigmoid_gate, gated_add, add, gelu, silu      src/model/ops.ts:101-113
   matmul_fp8 / matmul_bf16 / matmul_f32 one-shots        src/kernels/matmul.ts:223-265
   unpack_fp8 one-shot   src/kernels/fp8.ts:24-36
+  Cache4                (additive) a key / value cache held in 4 bits: append, attention, evict (include/we_cache4.h)
 
 Every op runs the hand-written gfx950 kernels in libwe.so; there is no CPU fallback. Importing works
 without a GPU (the symbol checks use that); creating a Graph needs the library and a GPU and raises
@@ -26,6 +27,7 @@ import numpy as np
 PKG = pathlib.Path(__file__).resolve().parent
 LIB_PATH = PKG / "libwe.so"
 HEADER = PKG.parent / "include" / "we.h"
+CACHE4_HEADER = PKG.parent / "include" / "we_cache4.h"
 
 F32, F16, BF16, FP8, INT4 = 0, 1, 2, 3, 4
 DTYPES = {"f32": F32, "f16": F16, "bf16": BF16, "fp8": FP8, "int4": INT4}
@@ -68,6 +70,12 @@ class MatmulItem(ctypes.Structure):
     _fields_ = [("p", ctypes.POINTER(MatmulParams)), ("x", ctypes.c_void_p), ("w", ctypes.c_void_p),
                 ("y", ctypes.c_void_p), ("bias", ctypes.c_void_p), ("gate", ctypes.c_void_p),
                 ("residual", ctypes.c_void_p)]
+
+
+class Cache4Struct(ctypes.Structure):
+    """we_cache4: a 4-bit cache's shape and buffer."""
+    _fields_ = [("batch", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32), ("dim", ctypes.c_uint32),
+                ("capacity", ctypes.c_uint32), ("data", ctypes.c_void_p)]
 
 
 _P, _I, _U32, _U64, _SZ, _F, _I64 = (ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_size_t,
@@ -141,12 +149,21 @@ SIGNATURES = {
     "we_st_read": (_I, [_P, _U32, _U64, _U64, _P, _U32]),
 }
 
+# the 4-bit key / value cache (include/we_cache4.h)
+CACHE4_SIGNATURES = {
+    "we_cache4_bytes": (_I, [_P, _P, _P]),
+    "we_cache4_append": (_I, [_P, _P, _U32, _I, _P, _U32, _P, _U32, _P, _P, _P, _P, _P, _P, _P]),
+    "we_cache4_load": (_I, [_P, _P, _U32, _P, _P, _I, _P, _U32, _P, _U32]),
+    "we_cache4_attention": (_I, [_P, _P, _U32, _U32, _I, _I, _P, _U32, _P, _P, _U32, _P, _P, _P, _U32]),
+    "we_cache4_evict": (_I, [_P, _P, _U32, _P, _P, _U32, _P, _P, _P, _P, _P, _U32, _U32]),
+}
+
 _lib = None
 
 
-def header_functions():
-    """Names of every function declared in include/we.h."""
-    text = HEADER.read_text()
+def header_functions(header=HEADER):
+    """Names of every function declared in include/we.h (or another header)."""
+    text = header.read_text()
     return sorted(set(re.findall(r"^\s*(?:int|uint32_t|const char\*)\s+(we_\w+)\s*\(", text, re.M)))
 
 
@@ -159,7 +176,7 @@ def load_library(path=None):
     if not p.exists():
         raise RuntimeError(f"{p} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
     lib = ctypes.CDLL(str(p))
-    for name, (res, args) in SIGNATURES.items():
+    for name, (res, args) in {**SIGNATURES, **CACHE4_SIGNATURES}.items():
         fn = getattr(lib, name)
         fn.restype = res
         fn.argtypes = args
@@ -474,6 +491,34 @@ class Graph:
         self.check(self.lib.we_attention(self.ctx, tokens, heads, kv_heads, dim, 1 if causal else 0, dtype, _addr(q),
                                          q_stride, _addr(k), k_stride, _addr(v), v_stride, _addr(out), out_stride))
 
+    # the 4-bit key / value cache (include/we_cache4.h); `cache` is a Cache4, the arrays are device addresses or buffers
+    def cache4_append(self, cache, tokens, dtype, k, v, lens, lens_out, k_stride=0, v_stride=0, counts=None, seen=None,
+                      seen_out=None, pos=None, weight=None):
+        """we_cache4_append: K and V rows of `tokens` tokens per sequence into the slots from lens[b] on."""
+        self.check(self.lib.we_cache4_append(self.ctx, cache.ref, tokens, dtype, _addr(k), k_stride, _addr(v), v_stride,
+                                             _addr(counts), _addr(lens), _addr(lens_out), _addr(seen), _addr(seen_out),
+                                             _addr(pos), _addr(weight)))
+
+    def cache4_load(self, cache, tokens, dtype, k, v, first=None, lens=None, k_stride=0, v_stride=0):
+        """we_cache4_load: the stored values of `tokens` slots per sequence, from first[b] on."""
+        self.check(self.lib.we_cache4_load(self.ctx, cache.ref, tokens, _addr(first), _addr(lens), dtype, _addr(k),
+                                           k_stride, _addr(v), v_stride))
+
+    def cache4_attention(self, cache, tokens, heads, causal, dtype, q, lens, out, q_stride=0, out_stride=0, counts=None,
+                         max_len=0, weight=None, weight_out=None):
+        """we_cache4_attention: `tokens` queries per sequence over its slots; with weight_out the attention each slot
+        received is added to `weight`."""
+        self.check(self.lib.we_cache4_attention(self.ctx, cache.ref, tokens, heads, 1 if causal else 0, dtype, _addr(q),
+                                                q_stride, _addr(counts), _addr(lens), max_len, _addr(weight),
+                                                _addr(weight_out), _addr(out), out_stride))
+
+    def cache4_evict(self, cache, keep, lens, lens_out, weight, weight_out, pos, pos_out, seen=None, sinks=0, recent=0,
+                     max_len=0):
+        """we_cache4_evict: every sequence cut to at most `keep` slots, those of the lowest weight given up."""
+        self.check(self.lib.we_cache4_evict(self.ctx, cache.ref, keep, _addr(lens), _addr(lens_out), max_len,
+                                            _addr(weight), _addr(weight_out), _addr(pos), _addr(pos_out), _addr(seen),
+                                            sinks, recent))
+
     def elementwise(self, op, n, d, dtype, a, b, c, out):
         self.check(self.lib.we_elementwise(self.ctx, op, n, d, dtype, _addr(a), _addr(b), _addr(c), _addr(out)))
 
@@ -643,6 +688,55 @@ def attention(graph, q, k, v, shape, dtype=F32):
     out = graph.buffer(s.tokens * s.heads * s.dim * ELEM_BYTES[dtype])
     graph.attention(s.tokens, s.heads, s.kv_heads, s.dim, s.causal, dtype, q, k, v, out)
     return out
+
+
+class Cache4:
+    """A key / value cache held in 4 bits (include/we_cache4.h) for `batch` sequences of up to `capacity` slots: a shape and
+    its buffer, as the Graph.cache4_* calls take it. Without `data` (a device address, or a Buffer) it makes its buffer and
+    the arrays of a decoding program, which append(), attention() and evict() update in place: lens (slots in use), seen
+    (tokens so far), pos (the position of a slot's token) and weight (the attention a slot has received)."""
+
+    def __init__(self, graph, batch, kv_heads, dim, capacity, data=None):
+        self.graph, self.batch, self.kv_heads, self.dim, self.capacity = graph, batch, kv_heads, dim, capacity
+        self.struct = Cache4Struct(batch, kv_heads, dim, capacity, None)
+        self.ref = ctypes.byref(self.struct)
+        nbytes = ctypes.c_uint64()
+        graph.check(graph.lib.we_cache4_bytes(graph.ctx, self.ref, ctypes.byref(nbytes)))
+        self.nbytes = nbytes.value
+        self.data, self.lens, self.seen, self.pos, self.weight = data, None, None, None, None
+        if data is None:
+            self.data = graph.buffer(self.nbytes)
+            self.lens, self.seen = graph.buffer(batch * 4), graph.buffer(batch * 4)
+            self.pos, self.weight = (graph.buffer(batch * kv_heads * capacity * 4) for _ in range(2))
+        self.struct.data = _addr(self.data).value
+
+    def append(self, k, v, tokens, dtype=F32, k_stride=0, v_stride=0, counts=None):
+        """Stores `tokens` K and V rows per sequence (counts[b] of them) behind what it holds."""
+        self.graph.cache4_append(self, tokens, dtype, k, v, self.lens, self.lens, k_stride, v_stride, counts, self.seen,
+                                 self.seen, self.pos, self.weight)
+
+    def attention(self, q, tokens, heads, dtype=F32, causal=True, q_stride=0, counts=None, max_len=0, track=False):
+        """A new out [batch, tokens, heads, dim] of the newest `tokens` tokens' queries; `track`: the attention each slot
+        received is added to self.weight."""
+        if self.kv_heads == 0 or heads % self.kv_heads:
+            raise WeError(1, "heads must be a multiple of kvHeads")
+        out = self.graph.buffer(self.batch * tokens * heads * self.dim * ELEM_BYTES[dtype])
+        w = self.weight if track else None
+        self.graph.cache4_attention(self, tokens, heads, causal, dtype, q, self.lens, out, q_stride, 0, counts, max_len, w, w)
+        return out
+
+    def evict(self, keep, sinks=0, recent=0, max_len=0):
+        """Cuts every sequence to at most `keep` slots by self.weight; the first `sinks` and the last `recent` tokens stay."""
+        self.graph.cache4_evict(self, keep, self.lens, self.lens, self.weight, self.weight, self.pos, self.pos, self.seen,
+                                sinks, recent, max_len)
+
+    def free(self):
+        """Gives back the buffers that it made."""
+        if self.lens is not None:
+            for b in (self.data, self.lens, self.seen, self.pos, self.weight):
+                self.graph.free(b)
+            self.data = self.lens = self.seen = self.pos = self.weight = None
+            self.struct.data = None
 
 
 def _elementwise(graph, op, a, b, c, n, d=1, dtype=F32):
