@@ -1,5 +1,5 @@
-// A key / value cache held in 4 bits (include/we_cache4.h): append (quantize), load (dequantize), attention over it and
-// eviction by accumulated attention weight.
+// A key / value cache held in 4 bits (include/we_cache4.h): append (quantize), load (dequantize) and eviction by
+// accumulated attention weight. Attention over it: cache4_attention.hip.
 #include "common.h"
 #include "internal.h"
 
@@ -130,98 +130,6 @@ __global__ void __launch_bounds__(256) cache4_load_kernel(Cache4Load a, uint32_t
     for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf((float)(codes >> (4 * e) & 15u), s, m);  // code * scale is exact in f32
     store8<DT>(to, ((size_t)b * a.tokens + i) * (is_v ? a.v_stride : a.k_stride) + (size_t)h * dim + w * 8, x);
   }
-}
-
-// ------------------------------------------------------------------------------------------ attention
-struct AttnArgs4 {
-  Cache4Attention a;
-  uint32_t group;
-  float scale_log2;  // log2(e) / sqrt(dim)
-  float* lse;        // [batch, heads, tokens]: log2 of a row's sum of 2^score (weights only)
-};
-
-__device__ __forceinline__ float load_q(const Cache4Attention& a, size_t i) {
-  return a.dtype == F32 ? ((const float*)a.q)[i] : a.dtype == F16 ? load_as_f32<F16>(a.q, i) : load_as_f32<BF16>(a.q, i);
-}
-__device__ __forceinline__ uint32_t visible(const Cache4Attention& a, uint32_t len, uint32_t count, uint32_t i) {
-  const int32_t n = a.causal ? (int32_t)(len + i + 1) - (int32_t)count : (int32_t)len;
-  return n < 0 ? 0u : (uint32_t)n;
-}
-// q (in LDS) times the K row of a slot
-__device__ __forceinline__ float dot_slot(const Cache4Attention& a, const float* q, size_t slot) {
-  const uint32_t words = a.c.dim / 8;
-  float s = 0.0f;
-  for (uint32_t w = 0; w < words; w++) {
-    const uint32_t codes = ((const uint32_t*)a.c.kc)[slot * words + w], sm = a.c.ks[slot * (words / 8) + w / 8];
-    const float sc = f16_to_f32((uint16_t)sm), m = f16_to_f32((uint16_t)(sm >> 16));
-#pragma unroll
-    for (int e = 0; e < 8; e++) s = __builtin_fmaf(__builtin_fmaf((float)(codes >> (4 * e) & 15u), sc, m), q[w * 8 + e], s);
-  }
-  return s;
-}
-
-// One wave per query and head; 64 slots at a time, a lane per slot for the scores, a lane per value of V for the products.
-__global__ void __launch_bounds__(64) cache4_attention_kernel(AttnArgs4 g) {
-  const Cache4Attention& a = g.a;
-  __shared__ float q[256];
-  const uint32_t b = blockIdx.z, h = blockIdx.y, i = blockIdx.x, lane = threadIdx.x, dim = a.c.dim;
-  const uint32_t len = clamped(a.lens[b], a.max_len), count = a.counts ? clamped(a.counts[b], a.tokens) : a.tokens;
-  if (i >= count) return;
-  const size_t row = (size_t)b * a.tokens + i;
-  for (uint32_t d = lane; d < dim; d += 64) q[d] = load_q(a, row * a.q_stride + (size_t)h * dim + d);
-  __syncthreads();
-  const uint32_t n = visible(a, len, count, i);
-  const size_t base = ((size_t)b * a.c.kv_heads + h / g.group) * a.c.capacity;
-  float m = -3e38f, l = 0.0f, o[4] = {};
-  for (uint32_t k0 = 0; k0 < n; k0 += 64) {
-    const float s = k0 + lane < n ? dot_slot(a, q, base + k0 + lane) * g.scale_log2 : -INFINITY;
-    float mx = s;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) mx = fmaxf(mx, __shfl_xor(mx, x));
-    const float mn = fmaxf(m, mx), alpha = exp2f(m - mn), p = k0 + lane < n ? exp2f(s - mn) : 0.0f;
-    float sum = p;
-#pragma unroll
-    for (int x = 1; x < 64; x *= 2) sum += __shfl_xor(sum, x);
-    l = l * alpha + sum;
-    m = mn;
-    for (int j = 0; j < 4; j++) o[j] *= alpha;
-    const uint32_t kn = n - k0 < 64 ? n - k0 : 64;
-    for (uint32_t k = 0; k < kn; k++) {
-      const float pk = __shfl(p, (int)k);
-      const size_t slot = base + k0 + k;
-      for (uint32_t j = 0; j < dim / 64; j++) {
-        const uint32_t u = a.c.vc[slot * (dim / 2) + j * 32 + lane / 2] >> (4 * (lane & 1)) & 15u, sm = a.c.vs[slot * (dim / 64) + j];
-        o[j] = __builtin_fmaf(pk, __builtin_fmaf((float)u, f16_to_f32((uint16_t)sm), f16_to_f32((uint16_t)(sm >> 16))), o[j]);
-      }
-    }
-  }
-  for (uint32_t j = 0; j < dim / 64; j++) {
-    const float v = n ? o[j] / l : 0.0f;
-    const size_t at = row * a.out_stride + (size_t)h * dim + j * 64 + lane;
-    if (a.dtype == F32) ((float*)a.out)[at] = v;
-    else if (a.dtype == F16) store_from_f32<F16>(a.out, at, v);
-    else store_from_f32<BF16>(a.out, at, v);
-  }
-  if (g.lse && lane == 0) g.lse[((size_t)b * a.heads + h) * a.tokens + i] = m + log2f(l);
-}
-
-// A lane per slot of a kv head: its probabilities summed over the queries of the head's group.
-__global__ void __launch_bounds__(64) cache4_weight_kernel(AttnArgs4 g) {
-  const Cache4Attention& a = g.a;
-  __shared__ float q[256];
-  const uint32_t b = blockIdx.z, gh = blockIdx.y, k = blockIdx.x * 64 + threadIdx.x, dim = a.c.dim;
-  const uint32_t len = clamped(a.lens[b], a.max_len), count = a.counts ? clamped(a.counts[b], a.tokens) : a.tokens;
-  const size_t slot = ((size_t)b * a.c.kv_heads + gh) * a.c.capacity + k;
-  float sum = 0.0f;
-  for (uint32_t r = 0; r < count * g.group; r++) {
-    const uint32_t i = r / g.group, h = gh * g.group + r % g.group;
-    __syncthreads();
-    for (uint32_t d = threadIdx.x; d < dim; d += 64) q[d] = load_q(a, ((size_t)b * a.tokens + i) * a.q_stride + (size_t)h * dim + d);
-    __syncthreads();
-    if (k < visible(a, len, count, i))
-      sum += exp2f(dot_slot(a, q, slot) * g.scale_log2 - g.lse[((size_t)b * a.heads + h) * a.tokens + i]);
-  }
-  if (k < len) a.weight_out[slot] = (a.weight ? a.weight[slot] : 0.0f) + sum;
 }
 
 // ------------------------------------------------------------------------------------------ evict
@@ -376,18 +284,6 @@ hipError_t cache4_load_launch(const Cache4Load& L, hipStream_t s) {
   if (L.dtype == F32) hipLaunchKernelGGL(cache4_load_kernel<F32>, at, dim3(256), 0, s, L, (uint32_t)items);
   else if (L.dtype == F16) hipLaunchKernelGGL(cache4_load_kernel<F16>, at, dim3(256), 0, s, L, (uint32_t)items);
   else hipLaunchKernelGGL(cache4_load_kernel<BF16>, at, dim3(256), 0, s, L, (uint32_t)items);
-  return hipGetLastError();
-}
-
-size_t cache4_attention_scratch(const Cache4Attention& L) {
-  return L.weight_out ? (size_t)L.c.batch * L.heads * L.tokens * 4 : 0;
-}
-
-hipError_t cache4_attention_launch(const Cache4Attention& L, hipStream_t s) {
-  AttnArgs4 g{L, L.heads / L.c.kv_heads, 1.4426950408889634f / sqrtf((float)L.c.dim), (float*)L.scratch};
-  if (L.tokens) hipLaunchKernelGGL(cache4_attention_kernel, dim3(L.tokens, L.heads, L.c.batch), dim3(64), 0, s, g);
-  if (L.weight_out)
-    hipLaunchKernelGGL(cache4_weight_kernel, dim3((L.max_len + 63) / 64, L.c.kv_heads, L.c.batch), dim3(64), 0, s, g);
   return hipGetLastError();
 }
 
