@@ -29,7 +29,7 @@ extern "C" {
  * sequence's length is never used, whatever it is. */
 #define WE_CACHE4_GROUP 64
 typedef struct we_cache4 {
-  uint32_t batch;    /* sequences */
+  uint32_t batch;    /* sequences; batch * kv_heads at most 65535 */
   uint32_t kv_heads;
   uint32_t dim;      /* a multiple of 64, at most 256 */
   uint32_t capacity; /* slots of a sequence, a multiple of 64, at most 2^24 */

@@ -133,12 +133,13 @@ __global__ void __launch_bounds__(256) cache4_load_kernel(Cache4Load a, uint32_t
 }
 
 // ------------------------------------------------------------------------------------------ evict
-// One workgroup per sequence and kv head. The slots to give up are those below the n-th smallest (protected, weight, slot):
-// found digit by digit from the top in counts of the slots that share the digits fixed so far; then two passes in slot order
-// pair the holes with the survivors that fill them, and the rows move.
-struct EvictArgs {
-  Cache4Evict a;
-};
+// cache4_select_kernel: one workgroup per sequence and kv head finds which slots go and pairs the holes with the survivors
+// that fill them; the rows move there too when they are few, else in cache4_move_kernel over the whole chip. A slot's key is
+// (protected, weight as an ordered u32): 33 bits, of which the n-th smallest is found in three passes of 12, 11 and 10 bits
+// (counts of the slots that share the bits fixed so far). Reads 8 bytes a slot; bound by the latency of those passes. Up to
+// 32768 slots a wave holds its keys in registers and the passes run out of LDS; more are read again by each pass.
+constexpr int EV_NT = 1024, EV_WAVES = EV_NT / 64;
+constexpr uint32_t EV_FEW = 64;  // moves that the selecting workgroup does itself: one step of its 16-lane groups
 
 // f32 as a key of the same order: NaN highest, -0 as 0
 __device__ __forceinline__ uint32_t order_key(float w) {
@@ -147,106 +148,208 @@ __device__ __forceinline__ uint32_t order_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Exclusive sum over the 1024 threads' flags in thread order; `total` is the sum of all.
-__device__ __forceinline__ uint32_t block_rank(bool flag, uint32_t* waves, uint32_t& total) {
-  const uint64_t vote = __ballot(flag);
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  __syncthreads();
-  if (lane == 0) waves[wave] = (uint32_t)__popcll(vote);
-  __syncthreads();
-  uint32_t before = 0;
-  total = 0;
-  for (uint32_t w = 0; w < 16; w++) {
-    if (w < wave) before += waves[w];
-    total += waves[w];
+// One row from slot `at` to slot `to` (with the base of the unit), by the lanes j = 0 .. 4 NG + 3 of a group.
+template <int NG>
+__device__ __forceinline__ void move_row(const Cache4Evict& a, size_t to, size_t at, int j) {
+  if (j < 4 * NG) {
+    uint8_t* p = j < 2 * NG ? a.c.kc : a.c.vc;
+    const int o = (j < 2 * NG ? j : j - 2 * NG) * 16;
+    *(u32x4*)(p + to * (32 * NG) + o) = *(const u32x4*)(p + at * (32 * NG) + o);
+  } else if (j < 4 * NG + 2) {
+    uint32_t* p = j == 4 * NG ? a.c.ks : a.c.vs;
+#pragma unroll
+    for (int x = 0; x < NG; x++) p[to * NG + x] = p[at * NG + x];
+  } else if (j == 4 * NG + 2) {
+    a.weight_out[to] = a.weight[at];
+  } else if (j == 4 * NG + 3) {
+    a.pos_out[to] = a.pos[at];
   }
-  return before + (uint32_t)__popcll(vote & ((1ull << lane) - 1));
 }
+template <int NG>
+constexpr int kMoveLanes = NG <= 3 ? 16 : 32;
 
-__global__ void __launch_bounds__(1024) cache4_evict_kernel(EvictArgs g, uint32_t* from) {
+struct EvictArgs {
+  Cache4Evict a;
+  uint32_t most;     // moves of a unit at most
+  uint32_t* counts;  // more than EV_FEW: moves of a unit, and per unit its holes, then the slots that fill them
+  uint32_t* lists;
+  int late_lens;     // cache4_left_kernel writes lens_out
+};
+
+template <int NG, int VPT>
+__global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
   const Cache4Evict& a = g.a;
-  __shared__ uint32_t hist[256], waves[16], found[2];
-  const uint32_t gh = blockIdx.x, b = blockIdx.y, t = threadIdx.x, cap = a.c.capacity;
+  __shared__ uint32_t hist[4096], waves[3][EV_WAVES], found[2], few[2][EV_FEW];
+  const uint32_t gh = blockIdx.x, b = blockIdx.y, unit = b * a.c.kv_heads + gh, cap = a.c.capacity;
+  const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t len = clamped(a.lens[b], a.max_len), left = len < a.keep ? len : a.keep;
   const int64_t young = (int64_t)a.seen[b] - a.recent;
-  const size_t base = ((size_t)b * a.c.kv_heads + gh) * cap;
-  from += ((size_t)b * a.c.kv_heads + gh) * a.max_len;
-  auto prot = [&](uint32_t s) { const int32_t p = a.pos[base + s]; return p < (int32_t)a.sinks || p >= young; };
-  // the class the border falls into, and how many of it go
-  uint32_t open = 0;
-  for (uint32_t s0 = 0; s0 < len; s0 += 1024) {
-    uint32_t n;
-    block_rank(s0 + t < len && !prot(s0 + t), waves, n);
-    open += n;
-  }
-  uint32_t go = len - left;
-  const bool cls = go > open;
-  if (cls) go -= open;
-  uint32_t prefix = 0, mask = 0;
-  if (go) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
+  const float* weight = a.weight + (size_t)unit * cap;
+  const int32_t* pos = a.pos + (size_t)unit * cap;
+  if (!g.late_lens && gh == 0 && t == 0) a.lens_out[b] = (int32_t)left;
+
+  // the wave's pieces of 64 slots: v = 0 .. pieces - 1 from slot `from` on
+  const uint32_t pieces = ((len + 63) / 64 + EV_WAVES - 1) / EV_WAVES, from = wave * pieces * 64;
+  uint32_t key[VPT ? VPT : 1], safe[VPT ? (VPT + 31) / 32 : 1] = {};
+  auto load = [&](uint32_t v, uint32_t& k, bool& p) {
+    const uint32_t s = from + v * 64 + lane;
+    const bool in = s < len;
+    const int32_t at = in ? pos[s] : 0;
+    k = in ? order_key(weight[s]) : 0u;
+    p = at < (int32_t)a.sinks || at >= young;
+    return in;
+  };
+  // f(v, in, key, protected) for the wave's pieces
+  auto each = [&](auto&& f) {
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int v = 0; v < VPT; v++)
+        if ((uint32_t)v < pieces) f((uint32_t)v, from + v * 64 + lane < len, key[v], (safe[v / 32] >> (v % 32) & 1u) != 0);
+    } else {
+      for (uint32_t v = 0; v < pieces; v++) {
+        uint32_t k;
+        bool p;
+        const bool in = load(v, k, p);
+        f(v, in, k, p);
+      }
+    }
+  };
+  uint32_t moves = 0;
+  if (left < len) {
+    if constexpr (VPT > 0) {
+#pragma unroll
+      for (int v = 0; v < VPT; v++) {
+        bool p = false;
+        key[v] = 0;
+        if ((uint32_t)v < pieces) load((uint32_t)v, key[v], p);
+        safe[v / 32] |= (uint32_t)p << (v % 32);
+      }
+    }
+    // the border: its class and key, and how many of the slots that have them go
+    uint32_t go = len - left, prefix = 0;
+    bool cls = false;
+    auto narrow = [&](auto BITS, int shift, uint32_t mask) {
+      constexpr uint32_t bins = 1u << BITS;
       __syncthreads();
-      if (t < 256) hist[t] = 0;
+      for (uint32_t x = t; x < bins; x += EV_NT) hist[x] = 0;
       __syncthreads();
-      for (uint32_t s = t; s < len; s += 1024) {
-        const uint32_t k = order_key(a.weight[base + s]);
-        if (prot(s) == cls && (k & mask) == prefix) atomicAdd(&hist[k >> shift & 255u], 1u);
+      each([&](uint32_t, bool in, uint32_t k, bool p) {
+        const uint32_t d = mask ? k >> shift & (bins - 1) : k >> shift | (uint32_t)p << 11;
+        const bool mine = in && (mask == 0 || (p == cls && (k & mask) == prefix));
+        const uint64_t who = __ballot(mine);
+        if (!who) return;
+        // many slots have one key (nothing received yet): a wave of them adds once
+        const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(who));
+        if (__ballot(mine && d == d0) == who) {
+          if (lane == 0) atomicAdd(&hist[d0], (uint32_t)__popcll(who));
+        } else if (mine) {
+          atomicAdd(&hist[d], 1u);
+        }
+      });
+      __syncthreads();
+      // which bin the go-th falls into: each thread sums its bins, waves by lane exchange
+      constexpr uint32_t own = bins < EV_NT ? 1 : bins / EV_NT;
+      uint32_t c[own], sum = 0;
+#pragma unroll
+      for (uint32_t x = 0; x < own; x++) {
+        c[x] = t * own + x < bins ? hist[t * own + x] : 0;
+        sum += c[x];
+      }
+      uint32_t up = sum;
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) {
+        const uint32_t n = (uint32_t)__shfl_up((int)up, x);
+        up += lane >= (uint32_t)x ? n : 0;
+      }
+      if (lane == 63) waves[0][wave] = up;
+      __syncthreads();
+      uint32_t before = up - sum;
+      for (uint32_t w = 0; w < wave; w++) before += waves[0][w];
+#pragma unroll
+      for (uint32_t x = 0; x < own; x++) {
+        if (before < go && go <= before + c[x]) found[0] = t * own + x, found[1] = go - before;
+        before += c[x];
       }
       __syncthreads();
-      if (t == 0) {
-        uint32_t d = 0, n = go;
-        while (hist[d] < n) n -= hist[d++];
-        found[0] = d, found[1] = n;
+      go = found[1];
+      return found[0];
+    };
+    uint32_t d = narrow(std::integral_constant<int, 12>{}, 21, 0u);
+    cls = d >> 11;
+    prefix = d << 21;
+    d = narrow(std::integral_constant<int, 11>{}, 10, 0xffe00000u);
+    prefix |= d << 10;
+    d = narrow(std::integral_constant<int, 10>{}, 0, 0xfffffc00u);
+    prefix |= d;
+
+    // in slot order, so that ties go by slot and holes and survivors are numbered: a wave's slots are consecutive, and the
+    // waves before it have counted theirs
+    uint32_t ties = 0;
+    each([&](uint32_t, bool in, uint32_t k, bool p) { ties += (uint32_t)__popcll(__ballot(in && p == cls && k == prefix)); });
+    if (lane == 0) waves[0][wave] = ties;
+    __syncthreads();
+    ties = 0;
+    for (uint32_t w = 0; w < wave; w++) ties += waves[0][w];
+    const uint32_t first_tie = ties;
+    auto gone_of = [&](bool in, uint32_t k, bool p) {
+      const uint64_t tie = __ballot(in && p == cls && k == prefix);
+      const uint32_t rank = ties + (uint32_t)__popcll(tie & ((1ull << lane) - 1));
+      ties += (uint32_t)__popcll(tie);
+      return in && (p != cls ? cls : k < prefix || (k == prefix && rank < go));
+    };
+    uint32_t holes = 0, fills = 0;
+    each([&](uint32_t v, bool in, uint32_t k, bool p) {
+      const uint32_t s = from + v * 64 + lane;
+      const bool gone = gone_of(in, k, p);
+      holes += (uint32_t)__popcll(__ballot(gone && s < left));
+      fills += (uint32_t)__popcll(__ballot(in && !gone && s >= left));
+    });
+    if (lane == 0) waves[1][wave] = holes, waves[2][wave] = fills;
+    __syncthreads();
+    holes = fills = 0;
+    for (uint32_t w = 0; w < EV_WAVES; w++) {
+      if (w < wave) holes += waves[1][w], fills += waves[2][w];
+      moves += waves[1][w];
+    }
+    uint32_t* hole_list = g.most <= EV_FEW ? few[0] : g.lists + (size_t)unit * 2 * g.most;
+    uint32_t* fill_list = g.most <= EV_FEW ? few[1] : hole_list + g.most;
+    ties = first_tie;
+    each([&](uint32_t v, bool in, uint32_t k, bool p) {
+      const uint32_t s = from + v * 64 + lane;
+      const bool gone = gone_of(in, k, p), hole = gone && s < left, fill = in && !gone && s >= left;
+      const uint64_t h = __ballot(hole), f = __ballot(fill), below = (1ull << lane) - 1;
+      if (hole) hole_list[holes + (uint32_t)__popcll(h & below)] = s;
+      if (fill) fill_list[fills + (uint32_t)__popcll(f & below)] = s;
+      holes += (uint32_t)__popcll(h), fills += (uint32_t)__popcll(f);
+      if (in && !gone && s < left) {
+        if (a.weight_out != a.weight) a.weight_out[(size_t)unit * cap + s] = weight[s];
+        if (a.pos_out != a.pos) a.pos_out[(size_t)unit * cap + s] = pos[s];
       }
+    });
+    if (g.most <= EV_FEW) {
       __syncthreads();
-      prefix |= found[0] << shift, mask |= 255u << shift, go = found[1];
+      constexpr int L = kMoveLanes<NG>;
+      for (uint32_t m = t / L; m < moves; m += EV_NT / L)
+        move_row<NG>(a, (size_t)unit * cap + few[0][m], (size_t)unit * cap + few[1][m], (int)(t % L));
+    }
+  } else {
+    for (uint32_t s = t; s < len; s += EV_NT) {
+      if (a.weight_out != a.weight) a.weight_out[(size_t)unit * cap + s] = weight[s];
+      if (a.pos_out != a.pos) a.pos_out[(size_t)unit * cap + s] = pos[s];
     }
   }
-  // go: how many of the slots with the border's key go, the lowest first
-  uint32_t equal = 0, holes = 0, moves = 0;
-  for (uint32_t s0 = 0; s0 < len; s0 += 1024) {
-    const uint32_t s = s0 + t;
-    bool gone = false, tie = false;
-    if (s < len) {
-      const bool p = prot(s);
-      const uint32_t k = order_key(a.weight[base + s]);
-      gone = p != cls ? cls : go && k < prefix;
-      tie = p == cls && go && k == prefix;
-    }
-    uint32_t n;
-    const uint32_t rank = equal + block_rank(tie, waves, n);
-    equal += n;
-    gone |= tie && rank < go;
-    const bool hole = gone && s < left, move = !gone && s >= left && s < len;
-    const uint32_t hr = holes + block_rank(hole, waves, n);
-    holes += n;
-    const uint32_t mr = moves + block_rank(move, waves, n);
-    moves += n;
-    // holes come before every move's slot, so a list of holes below and of sources above fits one array
-    if (hole) from[hr] = s;
-    if (move) from[a.max_len - 1 - mr] = s;
-    if (s < left && !hole) {
-      a.weight_out[base + s] = a.weight[base + s];
-      a.pos_out[base + s] = a.pos[base + s];
-    }
-  }
-  __syncthreads();
-  for (uint32_t m = 0; m < moves; m++) {
-    const size_t to = base + from[m], at = base + from[a.max_len - 1 - m];
-    const uint32_t words = a.c.dim / 8;
-    if (t < words) {
-      ((uint32_t*)a.c.kc)[to * words + t] = ((uint32_t*)a.c.kc)[at * words + t];
-      ((uint32_t*)a.c.vc)[to * words + t] = ((uint32_t*)a.c.vc)[at * words + t];
-    }
-    if (t < words / 8) {
-      a.c.ks[to * (words / 8) + t] = a.c.ks[at * (words / 8) + t];
-      a.c.vs[to * (words / 8) + t] = a.c.vs[at * (words / 8) + t];
-    }
-    if (t == 0) {
-      a.weight_out[to] = a.weight[at];
-      a.pos_out[to] = a.pos[at];
-    }
-  }
+  if (g.most > EV_FEW && t == 0) g.counts[unit] = moves;
+}
+
+// Bound by HBM: a row is read and written once, 16 bytes a lane.
+template <int NG>
+__global__ void __launch_bounds__(256) cache4_move_kernel(EvictArgs g) {
+  constexpr uint32_t L = kMoveLanes<NG>;
+  const uint32_t unit = blockIdx.y, moves = g.counts[unit];
+  const uint32_t* holes = g.lists + (size_t)unit * 2 * g.most;
+  const size_t base = (size_t)unit * g.a.c.capacity;
+  for (uint32_t m = (blockIdx.x * 256 + threadIdx.x) / L; m < moves; m += gridDim.x * (256 / L))
+    move_row<NG>(g.a, base + holes[m], base + holes[g.most + m], (int)(threadIdx.x % L));
 }
 
 __global__ void __launch_bounds__(256) cache4_left_kernel(Cache4Evict a) {
@@ -254,6 +357,21 @@ __global__ void __launch_bounds__(256) cache4_left_kernel(Cache4Evict a) {
   if (b >= a.c.batch) return;
   const uint32_t len = clamped(a.lens[b], a.max_len);
   a.lens_out[b] = (int32_t)(len < a.keep ? len : a.keep);
+}
+
+template <int NG>
+void launch_evict(const EvictArgs& g, hipStream_t s) {
+  const Cache4Evict& a = g.a;
+  const dim3 units(a.c.kv_heads, a.c.batch);
+  if (a.max_len <= 8 * EV_NT) hipLaunchKernelGGL((cache4_select_kernel<NG, 8>), units, dim3(EV_NT), 0, s, g);
+  else if (a.max_len <= 32 * EV_NT) hipLaunchKernelGGL((cache4_select_kernel<NG, 32>), units, dim3(EV_NT), 0, s, g);
+  else hipLaunchKernelGGL((cache4_select_kernel<NG, 0>), units, dim3(EV_NT), 0, s, g);
+  if (g.most > EV_FEW) {
+    const uint32_t n = a.c.kv_heads * a.c.batch, per = 256 / kMoveLanes<NG>;
+    uint32_t blocks = (g.most + per - 1) / per;
+    const uint32_t fill = 4096 / n + 1;  // 16 workgroups a CU in all
+    hipLaunchKernelGGL(cache4_move_kernel<NG>, dim3(blocks < fill ? blocks : fill, n), dim3(256), 0, s, g);
+  }
 }
 
 uint32_t blocks_for(uint64_t items) {
@@ -287,11 +405,29 @@ hipError_t cache4_load_launch(const Cache4Load& L, hipStream_t s) {
   return hipGetLastError();
 }
 
-size_t cache4_evict_scratch(const Cache4Evict& L) { return (size_t)L.c.batch * L.c.kv_heads * L.max_len * 4; }
+namespace {
+uint32_t most_moves(const Cache4Evict& L) {
+  const uint32_t out = L.max_len > L.keep ? L.max_len - L.keep : 0;
+  return out < L.keep ? out : L.keep;
+}
+}  // namespace
+
+size_t cache4_evict_scratch(const Cache4Evict& L) {
+  const uint32_t most = most_moves(L);
+  return most <= EV_FEW ? 0 : (size_t)L.c.batch * L.c.kv_heads * (1 + 2 * (size_t)most) * 4;
+}
 
 hipError_t cache4_evict_launch(const Cache4Evict& L, hipStream_t s) {
-  hipLaunchKernelGGL(cache4_evict_kernel, dim3(L.c.kv_heads, L.c.batch), dim3(1024), 0, s, EvictArgs{L}, (uint32_t*)L.scratch);
-  hipLaunchKernelGGL(cache4_left_kernel, dim3((L.c.batch + 255) / 256), dim3(256), 0, s, L);
+  if ((uint64_t)L.c.batch * L.c.kv_heads > 65535) return hipErrorInvalidValue;
+  EvictArgs g{L, most_moves(L), (uint32_t*)L.scratch, (uint32_t*)L.scratch + (size_t)L.c.batch * L.c.kv_heads, L.lens_out == L.lens};
+  switch (L.c.dim / 64) {
+    case 1: launch_evict<1>(g, s); break;
+    case 2: launch_evict<2>(g, s); break;
+    case 3: launch_evict<3>(g, s); break;
+    default: launch_evict<4>(g, s); break;
+  }
+  // in place, the lengths change when every kv head has read them
+  if (g.late_lens) hipLaunchKernelGGL(cache4_left_kernel, dim3((L.c.batch + 255) / 256), dim3(256), 0, s, L);
   return hipGetLastError();
 }
 

@@ -1542,8 +1542,9 @@ int cache4_shape(we_ctx* ctx, const we_cache4* c) {
     return fail(ctx, WE_EUNSUPPORTED, "cache dim must be a multiple of %u and at most 256, got %u", WE_CACHE4_GROUP, c->dim);
   if (c->capacity == 0 || c->capacity % 64 || c->capacity > (1u << 24))
     return fail(ctx, WE_EINVAL, "cache capacity must be a multiple of 64 from 64 to %u, got %u", 1u << 24, c->capacity);
-  if (c->batch == 0 || c->batch > 65535 || c->kv_heads == 0 || c->kv_heads > 65535)
-    return fail(ctx, WE_EINVAL, "cache batch and kvHeads must be from 1 to 65535, got %u and %u", c->batch, c->kv_heads);
+  if (c->batch == 0 || c->kv_heads == 0 || (uint64_t)c->batch * c->kv_heads > 65535)
+    return fail(ctx, WE_EINVAL, "cache batch and kvHeads must be from 1 and their product at most 65535, got %u and %u", c->batch,
+                c->kv_heads);
   return WE_OK;
 }
 
