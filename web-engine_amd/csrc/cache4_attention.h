@@ -117,11 +117,28 @@ struct QRow {
   static constexpr float kCode = NP == 1 ? 0x1p-24f : 1.0f;  // what a code of key_operand stands for
 };
 
-// `src`: the row in memory or in LDS. F16 and BF16: their bits give the maximum, two values at a time (an infinity or a NaN
+// The values of a row that a lane needs, as they are stored.
+template <int NG, int NP, int PK>
+struct RawRow {
+  u32x4 v[NG][2 * PK * NP];
+};
+// `src`: the row in memory or in LDS; without `live` zeros
+template <int NG, int NP, int PK>
+__device__ __forceinline__ void fetch_row(bool live, const char* src, int c, RawRow<NG, NP, PK>& x) {
+#pragma unroll
+  for (int g = 0; g < NG; g++)
+#pragma unroll
+    for (int v = 0; v < 2 * PK * NP; v++) {
+      x.v[g][v] = u32x4{};
+      if (live) x.v[g][v] = ((const u32x4*)(src + (g * 64 + c % Cols<PK>::kQuarters * (16 * PK)) * (2 * NP)))[v];
+    }
+}
+
+// F16 and BF16: their bits give the maximum, two values at a time (an infinity or a NaN
 // counts as the largest finite value: it stays one in f16, in its own row); F32 below. The sums come from the operands, by
 // MFMAs against ones (16 for the odd codes, which the operand holds a sixteenth of).
 template <int NG, int NP, int PK>
-__device__ __forceinline__ void load_row(const Attn4& a, bool live, const char* src, int c, QRow<NG, NP, PK>& q) {
+__device__ __forceinline__ void make_row(const Attn4& a, const RawRow<NG, NP, PK>& raw, QRow<NG, NP, PK>& q) {
   constexpr int W = 8 * PK;  // words of 16-bit values a lane has of a group
   float up;
   // 2^e with the largest value 2^e in [2^13, 2^14); e in -98 .. 126, so that `unit` and 2^e are normal numbers
@@ -134,16 +151,9 @@ __device__ __forceinline__ void load_row(const Attn4& a, bool live, const char* 
   if constexpr (NP == 1) {
     uint32_t x[NG][W], big = 0;
 #pragma unroll
-    for (int g = 0; g < NG; g++) {
-      const char* i = src + (g * 64 + c % Cols<PK>::kQuarters * (16 * PK)) * 2;
+    for (int g = 0; g < NG; g++)
 #pragma unroll
-      for (int v = 0; v < W / 4; v++) {
-        u32x4 w = {};
-        if (live) w = ((const u32x4*)i)[v];
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[g][4 * v + e] = w[e];
-      }
-    }
+      for (int e = 0; e < W; e++) x[g][e] = raw.v[g][e / 4][e % 4];
     typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     u16x2 top = {};
 #pragma unroll
@@ -186,20 +196,13 @@ __device__ __forceinline__ void load_row(const Attn4& a, bool live, const char* 
   } else {
     float x[NG][16 * PK], big = 0.0f;
 #pragma unroll
-    for (int g = 0; g < NG; g++) {
-      const char* i = src + (g * 64 + c % Cols<PK>::kQuarters * (16 * PK)) * 4;
+    for (int g = 0; g < NG; g++)
 #pragma unroll
-      for (int v = 0; v < 4 * PK; v++) {
-        f32x4 w = {};
-        if (live) w = ((const f32x4*)i)[v];
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          x[g][4 * v + e] = w[e];
-          const float y = fabsf(w[e]);
-          big = fmaxf(big, y < INFINITY ? y : 0.0f);  // an infinite or NaN value stays one in f16, in its own row
-        }
+      for (int e = 0; e < 16 * PK; e++) {
+        x[g][e] = __uint_as_float(raw.v[g][e / 4][e % 4]);
+        const float y = fabsf(x[g][e]);
+        big = fmaxf(big, y < INFINITY ? y : 0.0f);  // an infinite or NaN value stays one in f16, in its own row
       }
-    }
     scale(__float_as_uint(row_max(big)) >> 23, 126);
 #pragma unroll
     for (int g = 0; g < NG; g++)
@@ -364,7 +367,7 @@ struct Ring {
 
 // RT blocks of 16 rows (PK 1), or 16 / PK rows (RT 1)
 template <int NG, int RT, int NP, int PK>
-__global__ void __launch_bounds__(64 * NW, 1) cache4_attention_kernel(Attn4 a) {
+__global__ void __launch_bounds__(64 * NW, NG <= 2 ? 2 : 1) cache4_attention_kernel(Attn4 a) {
   using R = Ring<NG>;
   using C = Cols<PK>;
   static_assert(RT == 1 || PK == 1, "blocks of rows are whole");
@@ -446,7 +449,9 @@ __global__ void __launch_bounds__(64 * NW, 1) cache4_attention_kernel(Attn4 a) {
     const bool live = row < rows;
     const uint32_t i = live ? row / a.group : 0, h = live ? row % a.group : 0;
     const char* src = RT == 1 ? ring + R::kBytes + r % C::kRows * (kPieces * 16) : q_at<NG, NP>(a, b, gh, i, h);
-    load_row<NG, NP, PK>(a, live && rt == cs, src, c, q[I]);
+    RawRow<NG, NP, PK> raw;
+    fetch_row<NG, NP, PK>(live && rt == cs, src, c, raw);
+    make_row<NG, NP, PK>(a, raw, q[I]);
     vis[I] = live ? sees(a, len, count, i) : len;
     m[I] = kNone, le[I] = lo[I] = 0.0f;
     static_for<0, NG>([&](auto G) { me[I][G] = mo[I][G] = 0.0f; });
@@ -556,22 +561,30 @@ __global__ void __launch_bounds__(64 * NW, 1) cache4_attention_kernel(Attn4 a) {
       // operand register i of product K: slots i of tiles 2 K and 2 K + 1
       u32x4 pf[RT][2][NP];
       static_for<0, RT>([&](auto I) {
-        static_for<0, C::kTiles>([&](auto X) {
-          static_for<0, 4>([&](auto E) {
-            const float p = s[I][X][E()];
-            uint32_t w = vw[X][E * NG + G];
-            if constexpr (MASK) w = k0 + 16 * PK * X + E < vis[I] ? w : 0u;  // p is 0 there; the scale may be anything
-            float& mn = E & 1 ? mo[I][G] : me[I][G];
-            mn = __builtin_fmaf(p, middle_of(w), mn);
-            const float ps = __builtin_fmaf(p, scale_of(w), zero);
-            uint32_t h[NP];
-            h[0] = f32_to_f16(ps);
-            if constexpr (NP == 2) h[1] = f32_to_f16(ps - f16_to_f32((uint16_t)h[0]));
-            static_for<0, NP>([&](auto P) {
-              if constexpr (PK == 1) {
-                if constexpr (X % 2 == 0) pf[I][X / 2][P][E()] = h[P];
-                else pf[I][X / 2][P][E()] |= h[P] << 16;
-              } else {
+        // p s of the lane's slot i of tile X, with p's part of the minima
+        auto weighted = [&](auto X, auto E) {
+          const float p = s[I][X][E()];
+          uint32_t w = vw[X][E * NG + G];
+          if constexpr (MASK) w = k0 + 16 * PK * X + E < vis[I] ? w : 0u;  // p is 0 there; the scale may be anything
+          float& mn = E & 1 ? mo[I][G] : me[I][G];
+          mn = __builtin_fmaf(p, middle_of(w), mn);
+          return __builtin_fmaf(p, scale_of(w), zero);
+        };
+        static_for<0, 4>([&](auto E) {
+          if constexpr (PK == 1) {
+            static_for<0, 2>([&](auto K) {
+              const float p0 = weighted(std::integral_constant<int, 2 * K>{}, E), p1 = weighted(std::integral_constant<int, 2 * K + 1>{}, E);
+              const f16x2 h = {(_Float16)p0, (_Float16)p1};
+              pf[I][K][0][E()] = __builtin_bit_cast(uint32_t, h);
+              if constexpr (NP == 2) pf[I][K][1][E()] = pack2(p0 - (float)h[0], p1 - (float)h[1], std::true_type{});
+            });
+          } else {
+            static_for<0, C::kTiles>([&](auto X) {
+              const float ps = weighted(X, E);
+              uint32_t h[NP];
+              h[0] = f32_to_f16(ps);
+              if constexpr (NP == 2) h[1] = f32_to_f16(ps - f16_to_f32((uint16_t)h[0]));
+              static_for<0, NP>([&](auto P) {
                 const uint32_t v = h[P] << (16 * (rt & 1));
                 if constexpr (PK == 2) {
                   pf[I][X][P][E()] = v;
@@ -579,9 +592,9 @@ __global__ void __launch_bounds__(64 * NW, 1) cache4_attention_kernel(Attn4 a) {
                   pf[I][0][P][E()] = rt < 2 ? v : 0u;
                   pf[I][1][P][E()] = rt < 2 ? 0u : v;
                 }
-              }
+              });
             });
-          });
+          }
         });
       });
       static_for<0, 4>([&](auto D) {
@@ -599,15 +612,19 @@ __global__ void __launch_bounds__(64 * NW, 1) cache4_attention_kernel(Attn4 a) {
     });
   };
 
-  for (int stage = 0; t < t1; t += NW, stage ^= 1) {
+  // the tiles that every row sees whole, then those at the rows' ends
+  int stage = 0;
+  auto step = [&](auto MASK) {
     if (t + NW < t1) wait_loads<R::kLoads>();
     else wait_loads<0>();
-    const char* st = ring + stage * R::kBytes;
-    if (t * 64 + 64 > least) tile(t, st, std::true_type{});
-    else tile(t, st, std::false_type{});
+    tile(t, ring + stage * R::kBytes, MASK);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the stage's reads are done before it is filled again
     if (t + 2 * NW < t1) issue(t + 2 * NW, stage);
-  }
+    t += NW, stage ^= 1;
+  };
+  const uint32_t whole = t1 < least / 64 ? t1 : least / 64;
+  while (t < whole) step(std::false_type{});
+  while (t < t1) step(std::true_type{});
 
   // join the waves, and a row's PK columns: the largest maximum, all sums brought to it, their total
   float* ml = (float*)lds;                         // [wave][16][2]
@@ -665,10 +682,10 @@ __device__ __forceinline__ void join_row(const Attn4& a, uint32_t ur) {
   constexpr int DIM = 64 * NG, LANES = DIM / 4, SIDE = 64 * NW / LANES;
   __shared__ f32x4 sums[SIDE][LANES];
   const uint32_t unit = ur / a.rows, row = ur % a.rows;
+  const uint32_t first = a.shares[unit * 2], n = a.shares[unit * 2 + 1];
   uint32_t len, count;
   unit_of(a, unit, len, count);
   if (row >= count * a.group) return;
-  const uint32_t first = a.shares[unit * 2], n = a.shares[unit * 2 + 1];
   const size_t at = ((size_t)(row / a.block_rows) * a.split_slots + first) * a.block_rows + row % a.block_rows;
   const uint32_t lane = threadIdx.x & 63;
   float top = kNone, l = 0.0f;
@@ -747,11 +764,14 @@ __device__ __forceinline__ void receive_scores(const Attn4& a, uint32_t unit, ui
     if (k + e < len) a.weight_out[slot + e] = (a.weight ? a.weight[slot + e] : 0.0f) + sum[e];
 }
 
-// The attention each slot received, from the cache: a wave takes 64 slots and walks the query rows, 16 at a time, with their sums known. No
-// slot is written by two waves, and the rows are added in one order.
+// The attention each slot received, from the cache: a workgroup takes 64 slots and its waves the query rows, every NW-th
+// 16 each, with their sums known and the next 16 on their way. No slot is written by two workgroups, and the rows are added in
+// one order.
 template <int NG, int NP>
 __device__ __forceinline__ void receive(const Attn4& a, uint32_t unit, uint32_t tile) {
+  __shared__ float sums[NW][64];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t b = unit / a.kv_heads, gh = unit % a.kv_heads;
   uint32_t len, count;
   unit_of(a, unit, len, count);
@@ -768,39 +788,55 @@ __device__ __forceinline__ void receive(const Attn4& a, uint32_t unit, uint32_t 
     });
   });
   const uint32_t rows = count * a.group;
-  // the first row that sees a slot of the wave's
+  // the first row that sees a slot of the tile
   const uint32_t from = a.causal && k0 + count > len ? (k0 + count - len) * a.group : 0;
   float sum[16], zero = 0.0f;
   asm("" : "+v"(zero));
   for (int x = 0; x < 16; x++) sum[x] = 0.0f;
-  for (uint32_t row0 = from / 16 * 16; row0 < rows; row0 += 16) {
+  RawRow<NG, NP, 1> raw;
+  float lse = 0.0f;
+  uint32_t vis = 0;
+  auto fetch = [&](uint32_t row0) {
     const uint32_t row = row0 + r;
     const bool live = row < rows;
     const uint32_t i = live ? row / a.group : 0, h = live ? row % a.group : 0;
+    fetch_row<NG, NP, 1>(live, q_at<NG, NP>(a, b, gh, i, h), c, raw);
+    vis = live ? sees(a, len, count, i) : 0;
+    lse = row_lse(a, unit, live ? row : 0, c);
+  };
+  uint32_t row0 = from / 16 * 16 + wave * 16;
+  if (row0 < rows) fetch(row0);
+  for (; row0 < rows; row0 += 16 * NW) {
     QRow<NG, NP, 1> q;
-    load_row<NG, NP, 1>(a, live, q_at<NG, NP>(a, b, gh, i, h), c, q);
-    const uint32_t vis = live ? sees(a, len, count, i) : 0;
-    const float lse = row_lse(a, unit, live ? row : 0, c);
+    make_row<NG, NP, 1>(a, raw, q);
+    const uint32_t end = vis;
+    const float sub = lse;
+    if (row0 + 16 * NW < rows) fetch(row0 + 16 * NW);
     static_for<0, 4>([&](auto T) {
       const f32x4 s = scores<NG, NP, 1>(kw[T], sw[T], q, zero);
       static_for<0, 4>([&](auto E) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[E()], q.unit, -lse));
-        sum[4 * T + E] += k0 + 16 * T + 4 * c + E < vis ? p : 0.0f;
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[E()], q.unit, -sub));
+        sum[4 * T + E] += k0 + 16 * T + 4 * c + E < end ? p : 0.0f;
       });
     });
   }
-  float mine = 0.0f;  // lane r of a quarter writes its slot 16 (r / 4) + 4 c + r % 4
+  float mine = 0.0f;  // lane r of a quarter has its slot 16 (r / 4) + 4 c + r % 4
   static_for<0, 16>([&](auto X) {
     float v = sum[X];
     for (int x = 1; x < 16; x *= 2) v += __shfl_xor(v, x);
     mine = r == X ? v : mine;
   });
-  const uint32_t k = 16 * (r / 4) + 4 * c + r % 4;
-  if (k0 + k < len) a.weight_out[slot + k] = (a.weight ? a.weight[slot + k] : 0.0f) + mine;
+  sums[wave][16 * (r / 4) + 4 * c + r % 4] = mine;
+  __syncthreads();
+  if (threadIdx.x >= 64 || k0 + threadIdx.x >= len) return;
+  mine = 0.0f;
+#pragma unroll
+  for (int w = 0; w < NW; w++) mine += sums[w][threadIdx.x];
+  a.weight_out[slot + threadIdx.x] = (a.weight ? a.weight[slot + threadIdx.x] : 0.0f) + mine;
 }
 
-// What follows the attention kernel, in one launch: first a workgroup per row whose shares are to be joined, then one per NW
-// tiles of a unit whose slots receive weight.
+// What follows the attention kernel, in one launch: first a workgroup per row whose shares are to be joined, then those of a
+// unit's slots that receive weight.
 template <int NG, int NP>
 __global__ void __launch_bounds__(64 * NW) cache4_finish_kernel(Attn4 a, uint32_t joins, uint32_t tile_blocks) {
   if (blockIdx.x < joins) {
@@ -808,7 +844,7 @@ __global__ void __launch_bounds__(64 * NW) cache4_finish_kernel(Attn4 a, uint32_
   } else {
     const uint32_t x = blockIdx.x - joins;
     if (a.scores) receive_scores(a, x / tile_blocks, x % tile_blocks);
-    else receive<NG, NP>(a, x / tile_blocks, x % tile_blocks * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+    else receive<NG, NP>(a, x / tile_blocks, x % tile_blocks);
   }
 }
 
@@ -822,7 +858,7 @@ hipError_t launch_np(const Attn4& a, hipStream_t s) {
     else if (a.rt == 1) hipLaunchKernelGGL((cache4_attention_kernel<NG, 1, NP, 1>), grid, block, 0, s, a);
     else if constexpr (most_rows(NG) == 2) hipLaunchKernelGGL((cache4_attention_kernel<NG, 2, NP, 1>), grid, block, 0, s, a);
   }
-  const uint32_t joins = a.split_slots ? units * a.rows : 0, slots = 64 * NW * (a.scores ? 4 : 1);
+  const uint32_t joins = a.split_slots ? units * a.rows : 0, slots = a.scores ? 64 * NW * 4 : 64;
   const uint32_t tiles = a.weight_out ? (a.max_len + slots - 1) / slots : 0;
   if (joins || tiles) hipLaunchKernelGGL((cache4_finish_kernel<NG, NP>), dim3(joins + tiles * units), block, 0, s, a, joins, tiles);
   return hipGetLastError();

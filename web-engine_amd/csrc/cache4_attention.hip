@@ -55,7 +55,7 @@ size_t cache4_attention_scratch(const Cache4Attention& L) {
 hipError_t cache4_attention_launch(const Cache4Attention& L, hipStream_t s) {
   Attn4 a = plan_of(L);
   const uint64_t units = (uint64_t)L.c.batch * L.c.kv_heads;
-  if (units > 65535 || units * a.row_blocks > 0x7fffffffull || units * ((L.max_len + 255) / 256) + units * a.rows > 0x7fffffffull)
+  if (units > 65535 || units * a.row_blocks > 0x7fffffffull || units * ((L.max_len + 63) / 64) + units * a.rows > 0x7fffffffull)
     return hipErrorInvalidValue;
   a.kc = L.c.kc, a.ks = L.c.ks, a.vc = L.c.vc, a.vs = L.c.vs, a.q = L.q, a.out = L.out, a.counts = L.counts, a.lens = L.lens;
   a.weight = L.weight, a.weight_out = L.weight_out, a.batch = L.c.batch, a.tokens = L.tokens, a.heads = L.heads;
