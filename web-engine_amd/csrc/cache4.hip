@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(256) cache4_append_kernel(AppendArgs g) {
     }
   }
   if (!g.late_lens && blockIdx.x == 0) {
-    __syncthreads();  // in place, the one workgroup of the sequence has read its length
+    __syncthreads();  // in place, this is the sequence's only workgroup and has read its length
     if (threadIdx.x == 0) lens_update(a, b, len0, seen0);
   }
 }
@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(256) cache4_load_kernel(Cache4Load a, uint32_t
 // (counts of the slots that share the bits fixed so far). Reads 8 bytes a slot; bound by the latency of those passes. Up to
 // 32768 slots a wave holds its keys in registers and the passes run out of LDS; more are read again by each pass.
 constexpr int EV_NT = 1024, EV_WAVES = EV_NT / 64;
+constexpr uint32_t EV_ONE_BY_ONE = 4;  // slots to give up that are found one after the other
 constexpr uint32_t EV_FEW = 64;  // moves that the selecting workgroup does itself: one step of its 16-lane groups
 
 // f32 as a key of the same order: NaN highest, -0 as 0
@@ -179,26 +180,32 @@ struct EvictArgs {
 template <int NG, int VPT>
 __global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
   const Cache4Evict& a = g.a;
-  __shared__ uint32_t hist[4096], waves[3][EV_WAVES], found[2], few[2][EV_FEW];
+  __shared__ uint32_t hist[4096], waves[2][EV_WAVES], found[3], few[2][EV_FEW];
+  __shared__ uint64_t lowest[EV_WAVES];
   const uint32_t gh = blockIdx.x, b = blockIdx.y, unit = b * a.c.kv_heads + gh, cap = a.c.capacity;
   const uint32_t t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t len = clamped(a.lens[b], a.max_len), left = len < a.keep ? len : a.keep;
   const int64_t young = (int64_t)a.seen[b] - a.recent;
-  const float* weight = a.weight + (size_t)unit * cap;
-  const int32_t* pos = a.pos + (size_t)unit * cap;
+  const size_t base = (size_t)unit * cap;
+  const float* weight = a.weight + base;
+  const int32_t* pos = a.pos + base;
+  const bool copy = a.weight_out != a.weight || a.pos_out != a.pos;
+  auto stay = [&](uint32_t s) {
+    if (a.weight_out != a.weight) a.weight_out[base + s] = weight[s];
+    if (a.pos_out != a.pos) a.pos_out[base + s] = pos[s];
+  };
   if (!g.late_lens && gh == 0 && t == 0) a.lens_out[b] = (int32_t)left;
+  if (left == len) {
+    if (copy)
+      for (uint32_t s = t; s < len; s += EV_NT) stay(s);
+    if (g.most > EV_FEW && t == 0) g.counts[unit] = 0;
+    return;
+  }
 
   // the wave's pieces of 64 slots: v = 0 .. pieces - 1 from slot `from` on
   const uint32_t pieces = ((len + 63) / 64 + EV_WAVES - 1) / EV_WAVES, from = wave * pieces * 64;
   uint32_t key[VPT ? VPT : 1], safe[VPT ? (VPT + 31) / 32 : 1] = {};
-  auto load = [&](uint32_t v, uint32_t& k, bool& p) {
-    const uint32_t s = from + v * 64 + lane;
-    const bool in = s < len;
-    const int32_t at = in ? pos[s] : 0;
-    k = in ? order_key(weight[s]) : 0u;
-    p = at < (int32_t)a.sinks || at >= young;
-    return in;
-  };
+  auto safe_of = [&](int32_t p) { return p < (int32_t)a.sinks || p >= young; };
   // f(v, in, key, protected) for the wave's pieces
   auto each = [&](auto&& f) {
     if constexpr (VPT > 0) {
@@ -207,138 +214,201 @@ __global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
         if ((uint32_t)v < pieces) f((uint32_t)v, from + v * 64 + lane < len, key[v], (safe[v / 32] >> (v % 32) & 1u) != 0);
     } else {
       for (uint32_t v = 0; v < pieces; v++) {
-        uint32_t k;
-        bool p;
-        const bool in = load(v, k, p);
-        f(v, in, k, p);
+        const uint32_t s = from + v * 64 + lane, at = s < len ? s : len - 1;
+        f(v, s < len, order_key(weight[at]), safe_of(pos[at]));
       }
     }
   };
-  uint32_t moves = 0;
-  if (left < len) {
-    if constexpr (VPT > 0) {
+  if constexpr (VPT > 0) {
+    // eight pieces at a time, so that their loads go out together
 #pragma unroll
-      for (int v = 0; v < VPT; v++) {
-        bool p = false;
-        key[v] = 0;
-        if ((uint32_t)v < pieces) load((uint32_t)v, key[v], p);
-        safe[v / 32] |= (uint32_t)p << (v % 32);
+    for (int v0 = 0; v0 < VPT; v0 += 8) {
+      if ((uint32_t)v0 < pieces) {
+        float w[8];
+        int32_t p[8];
+#pragma unroll
+        for (int v = 0; v < 8; v++) {
+          const uint32_t s = from + (v0 + v) * 64 + lane, at = s < len ? s : len - 1;
+          w[v] = weight[at], p[v] = pos[at];
+        }
+#pragma unroll
+        for (int v = 0; v < 8; v++) {
+          key[v0 + v] = order_key(w[v]);
+          safe[v0 / 32] |= (uint32_t)safe_of(p[v]) << (v0 % 32 + v);
+        }
+      } else {
+#pragma unroll
+        for (int v = 0; v < 8; v++) key[v0 + v] = 0;
       }
     }
-    // the border: its class and key, and how many of the slots that have them go
-    uint32_t go = len - left, prefix = 0;
-    bool cls = false;
-    auto narrow = [&](auto BITS, int shift, uint32_t mask) {
-      constexpr uint32_t bins = 1u << BITS;
-      __syncthreads();
-      for (uint32_t x = t; x < bins; x += EV_NT) hist[x] = 0;
-      __syncthreads();
-      each([&](uint32_t, bool in, uint32_t k, bool p) {
-        const uint32_t d = mask ? k >> shift & (bins - 1) : k >> shift | (uint32_t)p << 11;
-        const bool mine = in && (mask == 0 || (p == cls && (k & mask) == prefix));
-        const uint64_t who = __ballot(mine);
-        if (!who) return;
-        // many slots have one key (nothing received yet): a wave of them adds once
-        const uint32_t d0 = (uint32_t)__builtin_amdgcn_readlane((int)d, __builtin_ctzll(who));
-        if (__ballot(mine && d == d0) == who) {
-          if (lane == 0) atomicAdd(&hist[d0], (uint32_t)__popcll(who));
-        } else if (mine) {
-          atomicAdd(&hist[d], 1u);
-        }
-      });
-      __syncthreads();
-      // which bin the go-th falls into: each thread sums its bins, waves by lane exchange
-      constexpr uint32_t own = bins < EV_NT ? 1 : bins / EV_NT;
-      uint32_t c[own], sum = 0;
+  }
+
+  uint32_t go = len - left, moves = 0;
+  if (go <= EV_ONE_BY_ONE) {
+    // one slot or a few (a decode step of a full cache): the lowest, then the lowest above it, ...
+    uint64_t last = 0;
+    uint32_t gone[EV_ONE_BY_ONE];
 #pragma unroll
-      for (uint32_t x = 0; x < own; x++) {
-        c[x] = t * own + x < bins ? hist[t * own + x] : 0;
-        sum += c[x];
-      }
-      uint32_t up = sum;
+    for (uint32_t n = 0; n < EV_ONE_BY_ONE; n++) {
+      gone[n] = ~0u;
+      if (n >= go) continue;
+      uint64_t best = ~0ull;
+      each([&](uint32_t v, bool in, uint32_t k, bool p) {
+        const uint64_t x = ((uint64_t)p << 56 | (uint64_t)k << 24 | (from + v * 64 + lane)) + 1;  // above 0, the first `last`
+        if (in && x > last && x < best) best = x;
+      });
 #pragma unroll
       for (int x = 1; x < 64; x *= 2) {
-        const uint32_t n = (uint32_t)__shfl_up((int)up, x);
-        up += lane >= (uint32_t)x ? n : 0;
+        const uint64_t y = __shfl_xor(best, x);
+        best = y < best ? y : best;
       }
-      if (lane == 63) waves[0][wave] = up;
       __syncthreads();
-      uint32_t before = up - sum;
-      for (uint32_t w = 0; w < wave; w++) before += waves[0][w];
+      if (lane == 0) lowest[wave] = best;
+      __syncthreads();
+      best = lowest[lane % EV_WAVES];
 #pragma unroll
-      for (uint32_t x = 0; x < own; x++) {
-        if (before < go && go <= before + c[x]) found[0] = t * own + x, found[1] = go - before;
-        before += c[x];
+      for (int x = 1; x < EV_WAVES; x *= 2) {
+        const uint64_t y = __shfl_xor(best, x);
+        best = y < best ? y : best;
       }
-      __syncthreads();
-      go = found[1];
-      return found[0];
+      last = best;
+      gone[n] = (uint32_t)(best - 1) & 0xffffffu;
+    }
+    auto is_gone = [&](uint32_t s) {
+      bool x = false;
+#pragma unroll
+      for (uint32_t n = 0; n < EV_ONE_BY_ONE; n++) x |= gone[n] == s;
+      return x;
     };
-    uint32_t d = narrow(std::integral_constant<int, 12>{}, 21, 0u);
-    cls = d >> 11;
-    prefix = d << 21;
-    d = narrow(std::integral_constant<int, 11>{}, 10, 0xffe00000u);
-    prefix |= d << 10;
-    d = narrow(std::integral_constant<int, 10>{}, 0, 0xfffffc00u);
-    prefix |= d;
+    if (copy)
+      for (uint32_t s = t; s < left; s += EV_NT)
+        if (!is_gone(s)) stay(s);
+    // the holes in order meet the slots from `left` on that stay
+    uint32_t fill = left, hole = 0;
+    for (uint32_t n = 0; n < go; n++) {
+      uint32_t next = ~0u;  // the lowest hole not yet filled
+#pragma unroll
+      for (uint32_t m = 0; m < EV_ONE_BY_ONE; m++) next = gone[m] < left && gone[m] >= hole && gone[m] < next ? gone[m] : next;
+      if (next == ~0u) break;
+      while (is_gone(fill)) fill++;
+      if (g.most <= EV_FEW) {
+        if (t / kMoveLanes<NG> == n) move_row<NG>(a, base + next, base + fill, (int)(t % kMoveLanes<NG>));
+      } else if (t == 0) {
+        uint32_t* list = g.lists + (size_t)unit * 2 * g.most;
+        list[n] = next, list[g.most + n] = fill;
+      }
+      hole = next + 1, fill++, moves++;
+    }
+    if (g.most > EV_FEW && t == 0) g.counts[unit] = moves;
+    return;
+  }
 
-    // in slot order, so that ties go by slot and holes and survivors are numbered: a wave's slots are consecutive, and the
-    // waves before it have counted theirs
-    uint32_t ties = 0;
+  // the border: its class and key, and how many of the slots that have them go
+  uint32_t prefix = 0;
+  bool cls = false;
+  auto narrow = [&](auto BITS, int shift, uint32_t mask) {
+    constexpr uint32_t bins = 1u << BITS;
+    __syncthreads();
+    for (uint32_t x = t; x < bins; x += EV_NT) hist[x] = 0;
+    __syncthreads();
+    each([&](uint32_t, bool in, uint32_t k, bool p) {
+      const uint32_t d = mask ? k >> shift & (bins - 1) : k >> shift | (uint32_t)p << 11;
+      if (in && (mask == 0 || (p == cls && (k & mask) == prefix))) atomicAdd(&hist[d], 1u);
+    });
+    __syncthreads();
+    // which bin the go-th falls into: each thread sums its bins, waves by lane exchange
+    constexpr uint32_t own = bins < EV_NT ? 1 : bins / EV_NT;
+    uint32_t c[own], sum = 0;
+#pragma unroll
+    for (uint32_t x = 0; x < own; x++) {
+      c[x] = t * own + x < bins ? hist[t * own + x] : 0;
+      sum += c[x];
+    }
+    uint32_t up = sum;
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) {
+      const uint32_t n = (uint32_t)__shfl_up((int)up, x);
+      up += lane >= (uint32_t)x ? n : 0;
+    }
+    if (lane == 63) waves[0][wave] = up;
+    __syncthreads();
+    uint32_t before = up - sum;
+#pragma unroll
+    for (uint32_t w = 0; w < EV_WAVES; w++) before += w < wave ? waves[0][w] : 0;
+#pragma unroll
+    for (uint32_t x = 0; x < own; x++) {
+      if (before < go && go <= before + c[x]) found[0] = t * own + x, found[1] = go - before, found[2] = c[x];
+      before += c[x];
+    }
+    __syncthreads();
+    go = found[1];
+    return found[0];
+  };
+  uint32_t d = narrow(std::integral_constant<int, 12>{}, 21, 0u);
+  cls = d >> 11;
+  prefix = d << 21;
+  d = narrow(std::integral_constant<int, 11>{}, 10, 0xffe00000u);
+  prefix |= d << 10;
+  d = narrow(std::integral_constant<int, 10>{}, 0, 0xfffffc00u);
+  prefix |= d;
+
+  // In slot order, so that holes and survivors are numbered: a wave's slots are consecutive, and the waves before it have
+  // counted theirs. Where not all slots with the border's key go, the lowest do: those are numbered first.
+  const bool all_ties = found[2] == go;
+  uint32_t ties = 0;
+  if (!all_ties) {
     each([&](uint32_t, bool in, uint32_t k, bool p) { ties += (uint32_t)__popcll(__ballot(in && p == cls && k == prefix)); });
+    __syncthreads();
     if (lane == 0) waves[0][wave] = ties;
     __syncthreads();
     ties = 0;
     for (uint32_t w = 0; w < wave; w++) ties += waves[0][w];
-    const uint32_t first_tie = ties;
-    auto gone_of = [&](bool in, uint32_t k, bool p) {
-      const uint64_t tie = __ballot(in && p == cls && k == prefix);
-      const uint32_t rank = ties + (uint32_t)__popcll(tie & ((1ull << lane) - 1));
-      ties += (uint32_t)__popcll(tie);
-      return in && (p != cls ? cls : k < prefix || (k == prefix && rank < go));
-    };
-    uint32_t holes = 0, fills = 0;
-    each([&](uint32_t v, bool in, uint32_t k, bool p) {
-      const uint32_t s = from + v * 64 + lane;
-      const bool gone = gone_of(in, k, p);
-      holes += (uint32_t)__popcll(__ballot(gone && s < left));
-      fills += (uint32_t)__popcll(__ballot(in && !gone && s >= left));
-    });
-    if (lane == 0) waves[1][wave] = holes, waves[2][wave] = fills;
-    __syncthreads();
-    holes = fills = 0;
-    for (uint32_t w = 0; w < EV_WAVES; w++) {
-      if (w < wave) holes += waves[1][w], fills += waves[2][w];
-      moves += waves[1][w];
-    }
-    uint32_t* hole_list = g.most <= EV_FEW ? few[0] : g.lists + (size_t)unit * 2 * g.most;
-    uint32_t* fill_list = g.most <= EV_FEW ? few[1] : hole_list + g.most;
-    ties = first_tie;
-    each([&](uint32_t v, bool in, uint32_t k, bool p) {
-      const uint32_t s = from + v * 64 + lane;
-      const bool gone = gone_of(in, k, p), hole = gone && s < left, fill = in && !gone && s >= left;
-      const uint64_t h = __ballot(hole), f = __ballot(fill), below = (1ull << lane) - 1;
-      if (hole) hole_list[holes + (uint32_t)__popcll(h & below)] = s;
-      if (fill) fill_list[fills + (uint32_t)__popcll(f & below)] = s;
-      holes += (uint32_t)__popcll(h), fills += (uint32_t)__popcll(f);
-      if (in && !gone && s < left) {
-        if (a.weight_out != a.weight) a.weight_out[(size_t)unit * cap + s] = weight[s];
-        if (a.pos_out != a.pos) a.pos_out[(size_t)unit * cap + s] = pos[s];
-      }
-    });
-    if (g.most <= EV_FEW) {
-      __syncthreads();
-      constexpr int L = kMoveLanes<NG>;
-      for (uint32_t m = t / L; m < moves; m += EV_NT / L)
-        move_row<NG>(a, (size_t)unit * cap + few[0][m], (size_t)unit * cap + few[1][m], (int)(t % L));
-    }
-  } else {
-    for (uint32_t s = t; s < len; s += EV_NT) {
-      if (a.weight_out != a.weight) a.weight_out[(size_t)unit * cap + s] = weight[s];
-      if (a.pos_out != a.pos) a.pos_out[(size_t)unit * cap + s] = pos[s];
-    }
   }
-  if (g.most > EV_FEW && t == 0) g.counts[unit] = moves;
+  const uint32_t first_tie = ties;
+  const uint64_t below = (1ull << lane) - 1;
+  auto gone_of = [&](bool in, uint32_t k, bool p) {
+    bool tie = k == prefix;
+    if (!all_ties) {
+      const uint64_t who = __ballot(in && p == cls && tie);
+      tie = tie && ties + (uint32_t)__popcll(who & below) < go;
+      ties += (uint32_t)__popcll(who);
+    }
+    return in && (p != cls ? cls : k < prefix || tie);
+  };
+  uint32_t holes = 0, fills = 0;
+  each([&](uint32_t v, bool in, uint32_t k, bool p) {
+    const uint32_t s = from + v * 64 + lane;
+    const bool gone = gone_of(in, k, p);
+    holes += (uint32_t)__popcll(__ballot(gone && s < left));
+    fills += (uint32_t)__popcll(__ballot(in && !gone && s >= left));
+  });
+  __syncthreads();
+  if (lane == 0) waves[0][wave] = holes, waves[1][wave] = fills;
+  __syncthreads();
+  holes = fills = 0;
+  for (uint32_t w = 0; w < EV_WAVES; w++) {
+    if (w < wave) holes += waves[0][w], fills += waves[1][w];
+    moves += waves[0][w];
+  }
+  uint32_t* hole_list = g.most <= EV_FEW ? few[0] : g.lists + (size_t)unit * 2 * g.most;
+  uint32_t* fill_list = g.most <= EV_FEW ? few[1] : hole_list + g.most;
+  ties = first_tie;
+  each([&](uint32_t v, bool in, uint32_t k, bool p) {
+    const uint32_t s = from + v * 64 + lane;
+    const bool gone = gone_of(in, k, p), hole = gone && s < left, fill = in && !gone && s >= left;
+    const uint64_t h = __ballot(hole), f = __ballot(fill);
+    if (hole) hole_list[holes + (uint32_t)__popcll(h & below)] = s;
+    if (fill) fill_list[fills + (uint32_t)__popcll(f & below)] = s;
+    holes += (uint32_t)__popcll(h), fills += (uint32_t)__popcll(f);
+    if (copy && in && !gone && s < left) stay(s);
+  });
+  if (g.most <= EV_FEW) {
+    __syncthreads();
+    constexpr int L = kMoveLanes<NG>;
+    for (uint32_t m = t / L; m < moves; m += EV_NT / L) move_row<NG>(a, base + few[0][m], base + few[1][m], (int)(t % L));
+  } else if (t == 0) {
+    g.counts[unit] = moves;
+  }
 }
 
 // Bound by HBM: a row is read and written once, 16 bytes a lane.
@@ -385,7 +455,8 @@ hipError_t cache4_append_launch(const Cache4Append& L, hipStream_t s) {
   const uint64_t items = (uint64_t)L.tokens * L.c.kv_heads * (L.c.dim / 8) * 2;
   if (items > 0xffffffffull - 4096 * 256) return hipErrorInvalidValue;
   const uint32_t grid = items <= 2048 ? 1 : blocks_for(items);
-  AppendArgs g{L, (uint32_t)items, grid > 1};
+  // in place, the lengths change when every workgroup of their sequence has read them
+  AppendArgs g{L, (uint32_t)items, grid > 1 && (L.lens_out == L.lens || L.seen_out == L.seen)};
   const dim3 at(grid, L.c.batch);
   if (L.dtype == F32) hipLaunchKernelGGL(cache4_append_kernel<F32>, at, dim3(256), 0, s, g);
   else if (L.dtype == F16) hipLaunchKernelGGL(cache4_append_kernel<F16>, at, dim3(256), 0, s, g);

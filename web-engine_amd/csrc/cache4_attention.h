@@ -363,6 +363,8 @@ template <int NG>
 struct Ring {
   static constexpr int kCodes = 2048 * NG, kScales = 256 * NG, kBytes = 2 * (kCodes + kScales), kStages = 2;
   static constexpr int kLoads = 4 * NG + 2;
+  template <int NP, int PK>
+  static constexpr int kQLoads = (16 / PK * 8 * NG * NP + 63) / 64;  // of the rows of q
 };
 
 // RT blocks of 16 rows (PK 1), or 16 / PK rows (RT 1)
@@ -375,7 +377,9 @@ __global__ void __launch_bounds__(64 * NW, NG <= 2 ? 2 : 1) cache4_attention_ker
   static_assert(NW * 16 * ROW * 4 + NW * 16 * 8 <= NW * R::kStages * R::kBytes, "the join fits the ring");
   constexpr uint32_t ROWS = RT * C::kRows;
   constexpr bool ONCE = PK > 1 || (RT == 1 && most_rows(NG) > 1);  // one row block: no other workgroup reads these slots
-  __shared__ __attribute__((aligned(1024))) char lds[NW * R::kStages * R::kBytes];
+  constexpr int kPieces = 8 * NG * NP;  // of 16 bytes, of a row of q
+  __shared__ __attribute__((aligned(1024))) char lds[NW * R::kStages * R::kBytes + (RT == 1 ? R::template kQLoads<NP, PK> * 1024 : 0)];
+  char* lds_q = lds + NW * R::kStages * R::kBytes;
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const int rt = r / C::kRows, cs = c / C::kQuarters;  // the column's tile, the quarter's
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -427,28 +431,24 @@ __global__ void __launch_bounds__(64 * NW, NG <= 2 ? 2 : 1) cache4_attention_ker
   uint32_t vis[RT];
   float m[RT], le[RT], lo[RT], me[RT][NG], mo[RT][NG];  // l and the sum of p (minimum + 8 scale): over even slots i, and odd ones / 16
   f32x4 o[RT][4 * NG];
-  // The rows of q come first, and with one block of them through the ring's second stage: the compiler knows nothing of the
-  // direct loads and would wait for all of them before it took a register load's result.
-  constexpr int kPieces = 8 * NG * NP;  // of 16 bytes, of a row
-  constexpr int kQLoads = (C::kRows * kPieces + 63) / 64;
+  // The rows of q come first, and with one block of them through LDS (every wave brings all of them to the same place): the
+  // compiler knows nothing of the direct loads and would wait for all of them before it took a register load's result.
   if constexpr (RT == 1) {
-    static_assert(RT > 1 || kQLoads * 1024 <= R::kBytes, "the rows fit a stage");
-    static_for<0, kQLoads>([&](auto J) {
+    static_for<0, R::template kQLoads<NP, PK>>([&](auto J) {
       const uint32_t p = J * 64 + lane, row = row0 + p / kPieces;
-      if (p < C::kRows * kPieces && row < rows) dma16g(q_at<NG, NP>(a, b, gh, row / a.group, row % a.group) + p % kPieces * 16, ring + R::kBytes + J * 1024);
+      if (p < C::kRows * kPieces && row < rows) dma16g(q_at<NG, NP>(a, b, gh, row / a.group, row % a.group) + p % kPieces * 16, lds_q + J * 1024);
     });
-    if (t < t1) {
-      issue(t, 0);
-      wait_loads<R::kLoads>();
-    } else {
-      wait_loads<0>();
-    }
+    if (t < t1) issue(t, 0);
+    if (t + NW < t1) issue(t + NW, 1);
+    if (t + NW < t1) wait_loads<2 * R::kLoads>();
+    else if (t < t1) wait_loads<R::kLoads>();
+    else wait_loads<0>();
   }
   static_for<0, RT>([&](auto I) {
     const uint32_t row = row0 + 16 * I + r % C::kRows;
     const bool live = row < rows;
     const uint32_t i = live ? row / a.group : 0, h = live ? row % a.group : 0;
-    const char* src = RT == 1 ? ring + R::kBytes + r % C::kRows * (kPieces * 16) : q_at<NG, NP>(a, b, gh, i, h);
+    const char* src = RT == 1 ? lds_q + r % C::kRows * (kPieces * 16) : q_at<NG, NP>(a, b, gh, i, h);
     RawRow<NG, NP, PK> raw;
     fetch_row<NG, NP, PK>(live && rt == cs, src, c, raw);
     make_row<NG, NP, PK>(a, raw, q[I]);
@@ -457,9 +457,8 @@ __global__ void __launch_bounds__(64 * NW, NG <= 2 ? 2 : 1) cache4_attention_ker
     static_for<0, NG>([&](auto G) { me[I][G] = mo[I][G] = 0.0f; });
     static_for<0, 4 * NG>([&](auto D) { o[I][D] = f32x4{}; });
   });
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // q has left the stage
   if (RT > 1 && t < t1) issue(t, 0);
-  if (t + NW < t1) issue(t + NW, 1);
+  if (RT > 1 && t + NW < t1) issue(t + NW, 1);
   float zero = 0.0f;
   asm("" : "+v"(zero));  // a product of a scale is one instruction when it adds something
 
@@ -736,6 +735,22 @@ __device__ __forceinline__ void receive_scores(const Attn4& a, uint32_t unit, ui
   unit_of(a, unit, len, count);
   const uint32_t rows = count * a.group, k = (block * 64 * NW + threadIdx.x) * 4;
   if (block * 64 * NW * 4 >= len) return;
+  f32x4 v[8];
+  auto fetch = [&](uint32_t r0) {
+#pragma unroll
+    for (int x = 0; x < 8; x++) {
+      const float* s = a.scores + ((size_t)unit * a.rows + r0 + x) * a.max_len + k;
+      v[x] = f32x4{};
+      if (r0 + x >= rows || k >= len) continue;
+      if (a.max_len % 4 == 0) {  // rows of scores are 16-byte aligned
+        v[x] = *(const f32x4*)s;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[x][e] = k + e < a.max_len ? s[e] : 0.0f;
+      }
+    }
+  };
+  fetch(0);
   if (rows && threadIdx.x < 64) {
     const uint32_t r = threadIdx.x & 15;
     const float v = row_lse(a, unit, r < rows ? r : 0, (int)(threadIdx.x >> 4));
@@ -744,19 +759,15 @@ __device__ __forceinline__ void receive_scores(const Attn4& a, uint32_t unit, ui
   __syncthreads();
   if (k >= len) return;
   f32x4 sum = {};
-  const float* s = a.scores + (size_t)unit * a.rows * a.max_len + k;
-  const bool whole = a.max_len % 4 == 0;  // rows of scores are 16-byte aligned
-  for (uint32_t r = 0; r < rows; r++, s += a.max_len) {
-    const uint32_t vis = sees(a, len, count, r / a.group);
-    f32x4 v = {};
-    if (whole) {
-      v = *(const f32x4*)s;
-    } else {
+  for (uint32_t r0 = 0; r0 < rows; r0 += 8) {
+    if (r0) fetch(r0);
 #pragma unroll
-      for (int e = 0; e < 4; e++) v[e] = k + e < a.max_len ? s[e] : 0.0f;
+    for (int x = 0; x < 8; x++) {
+      if (r0 + x >= rows) break;
+      const uint32_t vis = sees(a, len, count, (r0 + x) / a.group);
+#pragma unroll
+      for (int e = 0; e < 4; e++) sum[e] += k + e < vis ? __builtin_amdgcn_exp2f(v[x][e] - lse[r0 + x]) : 0.0f;
     }
-#pragma unroll
-    for (int e = 0; e < 4; e++) sum[e] += k + e < vis ? __builtin_amdgcn_exp2f(v[e] - lse[r]) : 0.0f;
   }
   const size_t slot = (size_t)unit * a.capacity + k;
 #pragma unroll
