@@ -96,7 +96,12 @@ __device__ __forceinline__ u32x4 centred_operand(uint32_t w) {
 }
 __device__ __forceinline__ float scale_of(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[0]; }
 __device__ __forceinline__ float minimum_of(uint32_t w) { return (float)__builtin_bit_cast(f16x2, w)[1]; }
-__device__ __forceinline__ float middle_of(uint32_t w) { return __builtin_fmaf(scale_of(w), 8.0f, minimum_of(w)); }
+// minimum + 8 scale: one instruction that reads both halves (written out, it became a conversion and a product)
+__device__ __forceinline__ float middle_of(uint32_t w) {
+  float r;
+  asm("v_fma_mix_f32 %0, %1, %2, %1 op_sel:[0,0,1] op_sel_hi:[1,0,1]" : "=v"(r) : "v"(w), "s"(8.0f));
+  return r;
+}
 
 // The 16 columns of a product hold PK * (16 / PK) query rows: with few rows (a decode step's 4 or 8 heads of a kv head) column
 // t * (16 / PK) + q is row q against the t-th of PK tiles of 16 slots. The k slots of lane quarter c then belong to tile
