@@ -193,6 +193,23 @@ export function rotate(graph: Graph, x: Binding, heads: number, rope: Rope, pair
 export function attention(graph: Graph, q: Binding, k: Binding, v: Binding,
                           shape: { tokens: number; heads: number; kvHeads: number; dim: number; causal?: boolean },
                           dtype?: DType): Buffer;
+/** A key / value cache held in 4 bits, with a decoding program's arrays (include/we_cache4.h). */
+export class Cache4 {
+  constructor(graph: Graph, batch: number, kvHeads: number, dim: number, capacity: number);
+  data: Buffer;
+  lens: Buffer;
+  seen: Buffer;
+  pos: Buffer;
+  weight: Buffer;
+  append(k: Binding, v: Binding, tokens: number, dtype?: DType,
+         opts?: { kStride?: number; vStride?: number; counts?: Binding | null }): void;
+  load(k: Binding | null, v: Binding | null, tokens: number, dtype?: DType,
+       opts?: { first?: Binding | null; kStride?: number; vStride?: number }): void;
+  attention(q: Binding, tokens: number, heads: number, dtype?: DType,
+            opts?: { causal?: boolean; qStride?: number; counts?: Binding | null; maxLen?: number; track?: boolean }): Buffer;
+  evict(keep: number, opts?: { sinks?: number; recent?: number; maxLen?: number }): void;
+  free(): void;
+}
 /** src/model/ops.ts:102-113 */
 export function swiglu(graph: Graph, gate: Binding, up: Binding, n: number, dtype?: DType): Buffer;
 export function sigmoidGate(graph: Graph, a: Binding, gate: Binding, n: number, dtype?: DType): Buffer;

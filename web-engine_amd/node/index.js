@@ -517,6 +517,58 @@ function attention(graph, q, k, v, shape, dtype = F32) {
   return out;
 }
 
+/**
+ * A key / value cache held in 4 bits (include/we_cache4.h) for `batch` sequences of up to `capacity` slots, and the arrays of
+ * a decoding program, which append, attention and evict update in place: lens (slots in use), seen (tokens so far), pos
+ * (the position of a slot's token) and weight (the attention a slot has received). No counterpart in the reference.
+ */
+class Cache4 {
+  constructor(graph, batch, kvHeads, dim, capacity) {
+    Object.assign(this, { graph, batch, kvHeads, dim, capacity });
+    this.data = graph.buffer(addon.cache4Bytes(graph.ctx, batch, kvHeads, dim, capacity));
+    this.lens = graph.buffer(batch * 4);
+    this.seen = graph.buffer(batch * 4);
+    this.pos = graph.buffer(batch * kvHeads * capacity * 4);
+    this.weight = graph.buffer(batch * kvHeads * capacity * 4);
+  }
+
+  _args() {
+    return [this.graph.ctx, this.batch, this.kvHeads, this.dim, this.capacity, ptrOf(this.data)];
+  }
+
+  /** Stores `tokens` K and V rows per sequence (counts[b] of them) behind what it holds. */
+  append(k, v, tokens, dtype = F32, { kStride = 0, vStride = 0, counts = null } = {}) {
+    addon.cache4Append(...this._args(), tokens, dtype, ptrOf(k), kStride, ptrOf(v), vStride, ptrOf(counts), ptrOf(this.lens),
+                       ptrOf(this.lens), ptrOf(this.seen), ptrOf(this.seen), ptrOf(this.pos), ptrOf(this.weight));
+  }
+
+  /** The stored values of `tokens` slots per sequence, from first[b] on, into k and v (either may be null). */
+  load(k, v, tokens, dtype = F32, { first = null, kStride = 0, vStride = 0 } = {}) {
+    addon.cache4Load(...this._args(), tokens, ptrOf(first), ptrOf(this.lens), dtype, ptrOf(k), kStride, ptrOf(v), vStride);
+  }
+
+  /** A new out [batch, tokens, heads, dim] of the newest tokens' queries; `track`: the attention each slot received is
+   * added to this.weight. */
+  attention(q, tokens, heads, dtype = F32, { causal = true, qStride = 0, counts = null, maxLen = 0, track = false } = {}) {
+    if (heads % this.kvHeads) throw new Error("heads must be a multiple of kvHeads");
+    const out = this.graph.buffer(this.batch * tokens * heads * this.dim * ELEM_BYTES[dtype]);
+    const w = track ? ptrOf(this.weight) : null;
+    addon.cache4Attention(...this._args(), tokens, heads, causal ? 1 : 0, dtype, ptrOf(q), qStride, ptrOf(counts),
+                          ptrOf(this.lens), maxLen, w, w, ptrOf(out), 0);
+    return out;
+  }
+
+  /** Cuts every sequence to at most `keep` slots by this.weight; the first `sinks` and the last `recent` tokens stay. */
+  evict(keep, { sinks = 0, recent = 0, maxLen = 0 } = {}) {
+    addon.cache4Evict(...this._args(), keep, ptrOf(this.lens), ptrOf(this.lens), maxLen, ptrOf(this.weight),
+                      ptrOf(this.weight), ptrOf(this.pos), ptrOf(this.pos), ptrOf(this.seen), sinks, recent);
+  }
+
+  free() {
+    for (const b of [this.data, this.lens, this.seen, this.pos, this.weight]) this.graph.free(b);
+  }
+}
+
 function elementwise(graph, op, inputs, n, d = 1, dtype = F32) {
   const out = graph.buffer(n * ELEM_BYTES[dtype]);
   graph.elementwise(op, n, d, dtype, inputs[0], inputs.length > 1 ? inputs[1] : null,
@@ -584,7 +636,7 @@ function readTensor(st, tensor, limit, dst, threads, offset = 0) {
 
 module.exports = {
   addon, Graph, F32, F16, BF16, FP8, INT4, DTYPES, EPI, OP, MUL, TUNE,
-  matmulParams, conv3x3Params, kSplitFor, linear, norm, noMod, rotate, attention,
+  matmulParams, conv3x3Params, kSplitFor, linear, norm, noMod, rotate, attention, Cache4,
   swiglu, sigmoidGate, gatedAdd, addBias, add, gelu, silu,
   SafetensorsError, readHeader, readTensor, registerKernels,
   lastError: (graph) => addon.lastError(graph ? graph.ctx : null),

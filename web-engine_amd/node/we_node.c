@@ -1,5 +1,5 @@
 /*
- * Node N-API (v8) addon over the C ABI of include/we.h: the binding a TypeScript host of the engine uses in
+ * Node N-API (v8) addon over the C ABI of include/we.h and we_cache4.h: the binding a TypeScript host of the engine uses in
  * place of its WebGPU Graph (src/gpu/graph.ts) to reach the MI355X kernels.
  *
  * Conventions of the JS side:
@@ -17,6 +17,7 @@
 #include <string.h>
 
 #include "we.h"
+#include "we_cache4.h"
 
 #define MAXARGS 20
 
@@ -918,6 +919,101 @@ static napi_value Attention(napi_env env, napi_callback_info info) {
   return status(env, ctx, we_attention(ctx, tokens, heads, kvh, dim, causal, dt, q, qs, k, ks, v, vs, out, os));
 }
 
+/* the 4-bit key / value cache (we_cache4.h): each call takes its shape and buffer as (batch, kvHeads, dim, capacity, data)
+ * after the context */
+static we_cache4 cache4_arg(args_t* a) {
+  we_cache4 c = {u32_arg(a, 1), u32_arg(a, 2), u32_arg(a, 3), u32_arg(a, 4), ptr_arg(a, 5)};
+  return c;
+}
+
+/* cache4Bytes(ctx | null, batch, kvHeads, dim, capacity) -> bytes */
+static napi_value Cache4Bytes(napi_env env, napi_callback_info info) {
+  args_t a;
+  if (!get_args(env, info, &a, 5)) return NULL;
+  we_ctx* ctx = ptr_arg(&a, 0);
+  we_cache4 c = cache4_arg(&a);
+  if (a.bad) return NULL;
+  uint64_t bytes = 0;
+  int rc = we_cache4_bytes(ctx, &c, &bytes);
+  if (rc != WE_OK) return status(env, ctx, rc);
+  return num(env, (double)bytes);
+}
+
+/* cache4Append(ctx, ...cache, tokens, dtype, k, kStride, v, vStride, counts, lens, lensOut, seen, seenOut, pos, weight) */
+static napi_value Cache4Append(napi_env env, napi_callback_info info) {
+  args_t a;
+  if (!get_args(env, info, &a, 19)) return NULL;
+  we_ctx* ctx = ptr_arg(&a, 0);
+  we_cache4 c = cache4_arg(&a);
+  uint32_t tokens = u32_arg(&a, 6);
+  int32_t dt = i32_arg(&a, 7);
+  void* k = ptr_arg(&a, 8);
+  uint32_t ks = u32_arg(&a, 9);
+  void* v = ptr_arg(&a, 10);
+  uint32_t vs = u32_arg(&a, 11);
+  void *counts = ptr_arg(&a, 12), *lens = ptr_arg(&a, 13), *lens_out = ptr_arg(&a, 14), *seen = ptr_arg(&a, 15);
+  void *seen_out = ptr_arg(&a, 16), *pos = ptr_arg(&a, 17), *weight = ptr_arg(&a, 18);
+  if (a.bad) return NULL;
+  return status(env, ctx, we_cache4_append(ctx, &c, tokens, dt, k, ks, v, vs, (const int32_t*)counts, (const int32_t*)lens,
+                                           (int32_t*)lens_out, (const int32_t*)seen, (int32_t*)seen_out, (int32_t*)pos,
+                                           (float*)weight));
+}
+
+/* cache4Load(ctx, ...cache, tokens, first, lens, dtype, k, kStride, v, vStride) */
+static napi_value Cache4Load(napi_env env, napi_callback_info info) {
+  args_t a;
+  if (!get_args(env, info, &a, 14)) return NULL;
+  we_ctx* ctx = ptr_arg(&a, 0);
+  we_cache4 c = cache4_arg(&a);
+  uint32_t tokens = u32_arg(&a, 6);
+  void *first = ptr_arg(&a, 7), *lens = ptr_arg(&a, 8);
+  int32_t dt = i32_arg(&a, 9);
+  void* k = ptr_arg(&a, 10);
+  uint32_t ks = u32_arg(&a, 11);
+  void* v = ptr_arg(&a, 12);
+  uint32_t vs = u32_arg(&a, 13);
+  if (a.bad) return NULL;
+  return status(env, ctx, we_cache4_load(ctx, &c, tokens, (const int32_t*)first, (const int32_t*)lens, dt, k, ks, v, vs));
+}
+
+/* cache4Attention(ctx, ...cache, tokens, heads, causal, dtype, q, qStride, counts, lens, maxLen, weight, weightOut, out,
+ * outStride) */
+static napi_value Cache4Attention(napi_env env, napi_callback_info info) {
+  args_t a;
+  if (!get_args(env, info, &a, 19)) return NULL;
+  we_ctx* ctx = ptr_arg(&a, 0);
+  we_cache4 c = cache4_arg(&a);
+  uint32_t tokens = u32_arg(&a, 6), heads = u32_arg(&a, 7);
+  int32_t causal = i32_arg(&a, 8), dt = i32_arg(&a, 9);
+  void* q = ptr_arg(&a, 10);
+  uint32_t qs = u32_arg(&a, 11);
+  void *counts = ptr_arg(&a, 12), *lens = ptr_arg(&a, 13);
+  uint32_t max_len = u32_arg(&a, 14);
+  void *weight = ptr_arg(&a, 15), *weight_out = ptr_arg(&a, 16), *out = ptr_arg(&a, 17);
+  uint32_t os = u32_arg(&a, 18);
+  if (a.bad) return NULL;
+  return status(env, ctx, we_cache4_attention(ctx, &c, tokens, heads, causal, dt, q, qs, (const int32_t*)counts,
+                                              (const int32_t*)lens, max_len, (const float*)weight, (float*)weight_out, out, os));
+}
+
+/* cache4Evict(ctx, ...cache, keep, lens, lensOut, maxLen, weight, weightOut, pos, posOut, seen, sinks, recent) */
+static napi_value Cache4Evict(napi_env env, napi_callback_info info) {
+  args_t a;
+  if (!get_args(env, info, &a, 17)) return NULL;
+  we_ctx* ctx = ptr_arg(&a, 0);
+  we_cache4 c = cache4_arg(&a);
+  uint32_t keep = u32_arg(&a, 6);
+  void *lens = ptr_arg(&a, 7), *lens_out = ptr_arg(&a, 8);
+  uint32_t max_len = u32_arg(&a, 9);
+  void *weight = ptr_arg(&a, 10), *weight_out = ptr_arg(&a, 11), *pos = ptr_arg(&a, 12), *pos_out = ptr_arg(&a, 13);
+  void* seen = ptr_arg(&a, 14);
+  uint32_t sinks = u32_arg(&a, 15), recent = u32_arg(&a, 16);
+  if (a.bad) return NULL;
+  return status(env, ctx, we_cache4_evict(ctx, &c, keep, (const int32_t*)lens, (int32_t*)lens_out, max_len,
+                                          (const float*)weight, (float*)weight_out, (const int32_t*)pos, (int32_t*)pos_out,
+                                          (const int32_t*)seen, sinks, recent));
+}
+
 static napi_value UnpackFp8(napi_env env, napi_callback_info info) {
   args_t a;
   if (!get_args(env, info, &a, 5)) return NULL;
@@ -1248,6 +1344,8 @@ static napi_value Init(napi_env env, napi_value exports) {
       {"stOpen", StOpen},         {"stClose", StClose},       {"stCount", StCount},
       {"stInfo", StInfo},         {"stFind", StFind},         {"stMetadataCount", StMetadataCount},
       {"stMetadataAt", StMetadataAt}, {"stRead", StRead},
+      {"cache4Bytes", Cache4Bytes}, {"cache4Append", Cache4Append}, {"cache4Load", Cache4Load},
+      {"cache4Attention", Cache4Attention}, {"cache4Evict", Cache4Evict},
   };
   for (size_t i = 0; i < sizeof fns / sizeof fns[0]; i++) {
     napi_value f;

@@ -207,6 +207,11 @@ def _addr(b):
     return ctypes.c_void_p(int(b))
 
 
+def _raw(b):
+    """_addr as the number ctypes converts by itself: for calls of a few microseconds, where making pointer objects shows"""
+    return b if b is None or b.__class__ is int else b.ptr if isinstance(b, Buffer) else int(b)
+
+
 class Graph:
     """Mirror of the reference's Graph (src/gpu/graph.ts:26-155) over one we_ctx: buffers stay on the GPU,
     work is queued in order on one compute stream, freed buffers are pooled by size and come back zeroed."""
@@ -495,28 +500,28 @@ class Graph:
     def cache4_append(self, cache, tokens, dtype, k, v, lens, lens_out, k_stride=0, v_stride=0, counts=None, seen=None,
                       seen_out=None, pos=None, weight=None):
         """we_cache4_append: K and V rows of `tokens` tokens per sequence into the slots from lens[b] on."""
-        self.check(self.lib.we_cache4_append(self.ctx, cache.ref, tokens, dtype, _addr(k), k_stride, _addr(v), v_stride,
-                                             _addr(counts), _addr(lens), _addr(lens_out), _addr(seen), _addr(seen_out),
-                                             _addr(pos), _addr(weight)))
+        self.check(self.lib.we_cache4_append(self.ctx, cache.ref, tokens, dtype, _raw(k), k_stride, _raw(v), v_stride,
+                                             _raw(counts), _raw(lens), _raw(lens_out), _raw(seen), _raw(seen_out),
+                                             _raw(pos), _raw(weight)))
 
     def cache4_load(self, cache, tokens, dtype, k, v, first=None, lens=None, k_stride=0, v_stride=0):
         """we_cache4_load: the stored values of `tokens` slots per sequence, from first[b] on."""
-        self.check(self.lib.we_cache4_load(self.ctx, cache.ref, tokens, _addr(first), _addr(lens), dtype, _addr(k),
-                                           k_stride, _addr(v), v_stride))
+        self.check(self.lib.we_cache4_load(self.ctx, cache.ref, tokens, _raw(first), _raw(lens), dtype, _raw(k),
+                                           k_stride, _raw(v), v_stride))
 
     def cache4_attention(self, cache, tokens, heads, causal, dtype, q, lens, out, q_stride=0, out_stride=0, counts=None,
                          max_len=0, weight=None, weight_out=None):
         """we_cache4_attention: `tokens` queries per sequence over its slots; with weight_out the attention each slot
         received is added to `weight`."""
-        self.check(self.lib.we_cache4_attention(self.ctx, cache.ref, tokens, heads, 1 if causal else 0, dtype, _addr(q),
-                                                q_stride, _addr(counts), _addr(lens), max_len, _addr(weight),
-                                                _addr(weight_out), _addr(out), out_stride))
+        self.check(self.lib.we_cache4_attention(self.ctx, cache.ref, tokens, heads, 1 if causal else 0, dtype, _raw(q),
+                                                q_stride, _raw(counts), _raw(lens), max_len, _raw(weight),
+                                                _raw(weight_out), _raw(out), out_stride))
 
     def cache4_evict(self, cache, keep, lens, lens_out, weight, weight_out, pos, pos_out, seen=None, sinks=0, recent=0,
                      max_len=0):
         """we_cache4_evict: every sequence cut to at most `keep` slots, those of the lowest weight given up."""
-        self.check(self.lib.we_cache4_evict(self.ctx, cache.ref, keep, _addr(lens), _addr(lens_out), max_len,
-                                            _addr(weight), _addr(weight_out), _addr(pos), _addr(pos_out), _addr(seen),
+        self.check(self.lib.we_cache4_evict(self.ctx, cache.ref, keep, _raw(lens), _raw(lens_out), max_len,
+                                            _raw(weight), _raw(weight_out), _raw(pos), _raw(pos_out), _raw(seen),
                                             sinks, recent))
 
     def elementwise(self, op, n, d, dtype, a, b, c, out):
