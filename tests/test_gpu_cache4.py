@@ -309,6 +309,39 @@ def test_regions_past_32_bit_offsets(scope):
     assert (np.abs(got - want) <= C.tolerance(want, bounds, we.F16)).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("dim,heads,kv,tokens,lens", [
+    (128, 8, 2, 1, [4100, 3, 0, 2100, 64]),      # shares of sequences of very different length, one of them empty
+    (64, 32, 8, 1, [3000] * 7),                  # rows of 4 heads; as many shares as fit
+    (256, 12, 2, 2, [2200, 2177]),               # 12 rows
+    (192, 5, 1, 3, [5000]),                      # 15 rows
+    (128, 6, 2, 9, [2500, 2049]),                # 27 rows: two blocks a wave, shared out
+    (256, 5, 1, 8, [2300]),                      # 40 rows in three row blocks, shared out
+])
+def test_attention_shared_out(scope, dtype, dim, heads, kv, tokens, lens):
+    rng = np.random.default_rng(dim + heads)
+    cap = (max(lens) + 63) // 64 * 64
+    c = filled(rng, len(lens), kv, dim, cap, lens)
+    q, qa = rows(rng, len(lens), tokens, heads, dim, dtype)
+    check_attention(scope, c, q, qa, lens, None, True, dtype)
+    check_attention(scope, c, q, qa, lens, None, False, dtype, max_len=max(lens) - 1)  # an odd row of scores
+
+
+def test_attention_pads_are_not_read(scope):
+    """Queries behind a sequence's count may hold anything; a call without tokens still writes weights."""
+    g, rng = scope, np.random.default_rng(17)
+    c = filled(rng, 2, 2, 128, 128, [90, 70])
+    q, qa = rows(rng, 2, 12, 4, 128, we.F16)
+    qa = qa.reshape(2, 12, -1)
+    qa[0, 5:], qa[1, 1:] = NAN_BITS[we.F16], NAN_BITS[we.F16]
+    q[0, 5:], q[1, 1:] = 0, 0
+    check_attention(g, c, q, qa, [90, 70], [5, 1], True, we.F16)
+    w = g.buffer(np.full(2 * 2 * 128, 2, np.float32))
+    g.cache4_attention(c.handle(g), 0, 4, True, we.F16, None, ints(g, [90, 70]), None, weight_out=w)
+    got = g.read(w, dtype=np.float32).reshape(2, 2, 128)
+    assert (got[0, :, :90] == 0).all() and (got[0, :, 90:] == 2).all() and (got[1, :, :70] == 0).all()
+
+
 # ---------------------------------------------------------------------------------------------------------- evict
 
 def evict_case(rng, batch, kv, cap, lens, kind):
@@ -336,6 +369,9 @@ def evict_case(rng, batch, kv, cap, lens, kind):
     (1, 1, 64, 64, [2], 1, 0, 0, "plain"),
     (2, 2, 128, 128, [100, 60], 99, 4, 10, "plain"),           # one slot of one sequence
     (2, 3, 192, 320, [300, 31], 64, 0, 0, "ties"),
+    (2, 1, 64, 128, [104, 103], 100, 2, 5, "zero"),            # four and three slots, found one by one, all of one weight
+    (2, 1, 128, 128, [105, 101], 100, 0, 0, "special"),        # five slots and one
+    (1, 2, 128, 2112, [2104], 2100, 3, 2099, "special"),       # four, most of them protected
     (1, 2, 256, 256, [256], 0, 0, 0, "plain"),                 # all of them
     (1, 2, 128, 256, [250], 100, 40, 80, "plain"),             # nearly all protected
     (1, 2, 128, 256, [250], 100, 60, 150, "plain"),            # more protected than may stay

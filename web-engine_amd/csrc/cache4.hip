@@ -453,7 +453,6 @@ uint32_t blocks_for(uint64_t items) {
 
 hipError_t cache4_append_launch(const Cache4Append& L, hipStream_t s) {
   const uint64_t items = (uint64_t)L.tokens * L.c.kv_heads * (L.c.dim / 8) * 2;
-  if (items > 0xffffffffull - 4096 * 256) return hipErrorInvalidValue;
   const uint32_t grid = items <= 2048 ? 1 : blocks_for(items);
   // in place, the lengths change when every workgroup of their sequence has read them
   AppendArgs g{L, (uint32_t)items, grid > 1 && (L.lens_out == L.lens || L.seen_out == L.seen)};
@@ -467,7 +466,6 @@ hipError_t cache4_append_launch(const Cache4Append& L, hipStream_t s) {
 
 hipError_t cache4_load_launch(const Cache4Load& L, hipStream_t s) {
   const uint64_t items = (uint64_t)L.tokens * L.c.kv_heads * (L.c.dim / 8) * 2;
-  if (items > 0xffffffffull - 4096 * 256) return hipErrorInvalidValue;
   if (!items) return hipSuccess;
   const dim3 at(blocks_for(items), L.c.batch);
   if (L.dtype == F32) hipLaunchKernelGGL(cache4_load_kernel<F32>, at, dim3(256), 0, s, L, (uint32_t)items);

@@ -266,7 +266,7 @@ __device__ __forceinline__ void unit_of(const Attn4& a, uint32_t unit, uint32_t&
   len = in_range(a.lens[b], a.max_len);
   count = a.counts ? in_range(a.counts[b], a.tokens) : a.tokens;
 }
-// How the tiles of all sequences are shared out: `chunk` tiles a workgroup, the least (and no fewer than kLeastTiles) with
+// How the tiles of all sequences are shared out: `chunk` tiles a workgroup, near the least (and no fewer than kLeastTiles) with
 // which the shares of all kv heads fit the slots. Lengths are on the device only, so every workgroup works it out, its lanes
 // a sequence each (at most kMostShared). A sequence without slots has one share, which writes its rows. Shares are numbered
 // sequence by sequence, kv head by kv head.
@@ -299,7 +299,7 @@ __device__ __forceinline__ bool share_of(const Attn4& a, uint32_t slot, Share& o
   }
   // (products of f32 here only choose among chunks that are all right; the share counts are exact)
   const float per = (float)a.kv_heads * __builtin_amdgcn_rcpf((float)a.split_slots);
-  uint32_t chunk = (uint32_t)((float)all * per);
+  uint32_t chunk = (uint32_t)((float)all * per) + 1;
   chunk = chunk > kLeastTiles ? chunk : kLeastTiles;
   for (;;) {  // ends: with a chunk of the longest sequence there are as many shares as units, and the slots are no fewer
     const float inv = __builtin_amdgcn_rcpf((float)chunk);
@@ -315,8 +315,7 @@ __device__ __forceinline__ bool share_of(const Attn4& a, uint32_t slot, Share& o
       }
     }
     if (all * a.kv_heads <= a.split_slots) break;
-    const uint32_t more = (uint32_t)((float)chunk * ((float)all * per - 1.0f));
-    chunk += more ? more : 1;
+    chunk += (uint32_t)((float)chunk * ((float)all * per - 1.0f) * 0.5f) + 1;  // half of what is too much
   }
   uint32_t before = 0;
 #pragma unroll

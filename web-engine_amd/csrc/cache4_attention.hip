@@ -5,7 +5,8 @@ namespace we {
 namespace {
 
 constexpr size_t kScoreBytes = 256u << 20;
-constexpr uint32_t kSlots = 512;  // workgroups that run at once: two a CU
+// workgroups that run at once: two a CU up to head dim 128, where their rings are 74 KB of its 160, one above
+uint32_t slots_of(uint32_t dim) { return dim <= 128 ? 512 : 256; }
 
 // rows a workgroup takes, and whether a sequence's tiles are shared out
 Attn4 plan_of(const Cache4Attention& L) {
@@ -16,9 +17,12 @@ Attn4 plan_of(const Cache4Attention& L) {
   a.block_rows = 16 * a.rt / a.pk;
   a.row_blocks = (a.rows + a.block_rows - 1) / a.block_rows;
   const uint64_t units = (uint64_t)L.c.batch * L.c.kv_heads, blocks = units * a.row_blocks;
-  // Shared out where the units alone leave half of the chip idle, and a sequence may be long enough for two shares
-  if (a.rows && blocks <= kSlots / 2 && L.c.batch <= kMostShared && (L.max_len + 63) / 64 >= 2 * kLeastTiles) {
-    a.split_slots = kSlots / a.row_blocks;
+  // Shared out where the units alone leave half of the chip idle and a sequence may have at least eight tiles for each of a
+  // workgroup's waves: fewer take less than the second launch and the sharing do (72 units of 17 tiles, f32: 9.8 us by a
+  // workgroup each, 13.2 us in three shares; 64 units of up to 64 tiles with weights: 25.9 us, 23.0 in shares)
+  const uint32_t slots = slots_of(L.c.dim);
+  if (a.rows && blocks <= slots / 2 && L.c.batch <= kMostShared && (L.max_len + 63) / 64 >= 8 * NW) {
+    a.split_slots = slots / a.row_blocks;
     a.split_slots = a.split_slots > units ? a.split_slots : (uint32_t)units;
   }
   return a;

@@ -1586,6 +1586,13 @@ int cache4_tokens(we_ctx* ctx, uint32_t tokens, int dtype, const char* what) {
   return WE_OK;
 }
 
+// append and load number the 8-value pieces of a sequence's K and V rows in 32 bits
+int cache4_pieces(we_ctx* ctx, const we_cache4* c, uint32_t tokens, const char* what) {
+  if ((uint64_t)tokens * c->kv_heads * (c->dim / 4) >= 0xf0000000ull)
+    return fail(ctx, WE_EINVAL, "%s takes fewer than 2^34 values of a sequence at once", what);
+  return WE_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1603,6 +1610,7 @@ int we_cache4_append(we_ctx* ctx, const we_cache4* cache, uint32_t tokens, int d
   we::Cache4Append L{};
   int rc = cache4_open(ctx, cache, &L.c);
   if (!rc) rc = cache4_tokens(ctx, tokens, dtype, "cache append");
+  if (!rc) rc = cache4_pieces(ctx, cache, tokens, "cache append");
   if (rc) return rc;
   if (!lens || !lens_out) return fail(ctx, WE_EINVAL, "cache lens or lens_out is null");
   if (seen_out && !seen) return fail(ctx, WE_EINVAL, "seen_out without seen");
@@ -1629,6 +1637,7 @@ int we_cache4_load(we_ctx* ctx, const we_cache4* cache, uint32_t tokens, const i
   we::Cache4Load L{};
   int rc = cache4_open(ctx, cache, &L.c);
   if (!rc) rc = cache4_tokens(ctx, tokens, dtype, "cache load");
+  if (!rc) rc = cache4_pieces(ctx, cache, tokens, "cache load");
   if (rc) return rc;
   if (!lens) return fail(ctx, WE_EINVAL, "cache lens is null");
   uint64_t kb = 0, vb = 0;
