@@ -327,6 +327,29 @@ def test_attention_shared_out(scope, dtype, dim, heads, kv, tokens, lens):
     check_attention(scope, c, q, qa, lens, None, False, dtype, max_len=max(lens) - 1)  # an odd row of scores
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_weights_of_few_rows_without_room_for_their_scores(scope, dtype):
+    """64 heads over a capacity of 2^20 + 64 slots: their scores would take more than 256 MB."""
+    g, rng = scope, np.random.default_rng(18)
+    cap = (1 << 20) + 64
+    h = we.Cache4(g, 1, 8, 64, cap, data=g.buffer(8 * cap * 72))
+    lens = ints(g, [700])
+    k, ka = rows(rng, 1, 700, 8, 64, we.F16)
+    v, va = rows(rng, 1, 700, 8, 64, we.F16)
+    g.cache4_append(h, 700, we.F16, g.buffer(ka), g.buffer(va), ints(g, [0]), lens)
+    c = C.Cache(1, 8, 64, 704)
+    c.put(0, 0, k[0], v[0])
+    q, qa = rows(rng, 1, 1, 64, 64, dtype)
+    o, w = g.buffer(qa.nbytes), g.buffer(8 * cap * 4)
+    g.cache4_attention(h, 1, 64, True, dtype, g.buffer(qa), lens, o, weight_out=w)
+    want, received, bounds = C.attention(c, q, [700], [1], True)
+    got = C.value(g.read(o, dtype=C.NP[dtype]).reshape(q.shape), dtype)
+    assert (np.abs(got - want) <= C.tolerance(want, bounds, dtype)).all()
+    gw = g.read(w, dtype=np.float32).reshape(8, cap)
+    assert (np.abs(gw[:, :700] - received[0, :, :700]) <= C.weight_tolerance(received, bounds)[0, :, :700] + gw[:, :700] * 2.0 ** -24).all()
+    assert not gw[:, 700:].any()
+
+
 def test_attention_pads_are_not_read(scope):
     """Queries behind a sequence's count may hold anything; a call without tokens still writes weights."""
     g, rng = scope, np.random.default_rng(17)

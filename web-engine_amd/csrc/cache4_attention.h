@@ -26,6 +26,11 @@ namespace we {
 constexpr int NW = 4;          // waves of a workgroup
 constexpr float kNone = -3e38f;  // the running maximum before the first score
 
+struct RowFacts {
+  float unit, sum[4];  // as in QRow
+  uint32_t sees;       // slots; 0: no row
+  uint32_t pad[2];
+};
 struct Attn4 {
   const uint8_t* kc;
   const uint32_t* ks;
@@ -50,6 +55,8 @@ struct Attn4 {
   uint32_t* shares;     // and each unit's first slot and its number of shares
   float* lse;           // weights, not shared out: [unit][rows], log2 of a row's sum of 2^score
   float* scores;        // weights of at most 16 rows: [unit][rows][max_len], the scores in log2 units
+  u32x4* operands;      // weights of more: the rows' operands [unit][16 rows][step and plane][lane]
+  RowFacts* facts;      // and the rest of them [unit][row, up to a multiple of 16]
 };
 hipError_t cache4_attention_64(const Attn4& a, hipStream_t s);
 hipError_t cache4_attention_128(const Attn4& a, hipStream_t s);
@@ -779,15 +786,42 @@ __device__ __forceinline__ void receive_scores(const Attn4& a, uint32_t unit, ui
     if (k + e < len) a.weight_out[slot + e] = (a.weight ? a.weight[slot + e] : 0.0f) + sum[e];
 }
 
+// The operands of all rows for `receive`, a wave per 16 of a unit. A launch of its own: written by the attention kernel, they
+// cost its loop more in registers (2048 queries over 8192 slots 380 -> 405 us) than the launch takes.
+template <int NG, int NP>
+__global__ void __launch_bounds__(64) cache4_operands_kernel(Attn4 a) {
+  const uint32_t blocks = (a.rows + 15) / 16, unit = blockIdx.x / blocks, row0 = blockIdx.x % blocks * 16;
+  const int lane = threadIdx.x, r = lane & 15, c = lane >> 4;
+  uint32_t len, count;
+  unit_of(a, unit, len, count);
+  const uint32_t row = row0 + r, rows = count * a.group;
+  if (row0 >= rows) return;
+  const bool live = row < rows;
+  const uint32_t i = live ? row / a.group : 0, h = live ? row % a.group : 0;
+  RawRow<NG, NP, 1> raw;
+  QRow<NG, NP, 1> q;
+  fetch_row<NG, NP, 1>(live, q_at<NG, NP>(a, unit / a.kv_heads, unit % a.kv_heads, i, h), c, raw);
+  make_row<NG, NP, 1>(a, raw, q);
+  static_for<0, NG>([&](auto G) {
+    static_for<0, 2>([&](auto S) {
+      static_for<0, NP>([&](auto P) { a.operands[(((size_t)blockIdx.x * NG + G) * 2 * NP + S * NP + P) * 64 + lane] = q.f[G][S][P]; });
+    });
+  });
+  if (c) return;
+  RowFacts f{};
+  f.unit = q.unit, f.sees = live ? sees(a, len, count, i) : 0;
+  static_for<0, NG>([&](auto G) { f.sum[G] = q.sum[G]; });
+  a.facts[(size_t)blockIdx.x * 16 + r] = f;
+}
+
 // The attention each slot received, from the cache: a workgroup takes 64 slots and its waves the query rows, every NW-th
-// 16 each, with their sums known and the next 16 on their way. No slot is written by two workgroups, and the rows are added in
+// 16 each, as operands, with their sums known and the next 16 on their way. No slot is written by two workgroups, and the rows are added in
 // one order.
 template <int NG, int NP>
 __device__ __forceinline__ void receive(const Attn4& a, uint32_t unit, uint32_t tile) {
   __shared__ float sums[NW][64];
   const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t b = unit / a.kv_heads, gh = unit % a.kv_heads;
   uint32_t len, count;
   unit_of(a, unit, len, count);
   const uint32_t k0 = tile * 64;
@@ -808,22 +842,25 @@ __device__ __forceinline__ void receive(const Attn4& a, uint32_t unit, uint32_t 
   float sum[16], zero = 0.0f;
   asm("" : "+v"(zero));
   for (int x = 0; x < 16; x++) sum[x] = 0.0f;
-  RawRow<NG, NP, 1> raw;
+  QRow<NG, NP, 1> next;
   float lse = 0.0f;
   uint32_t vis = 0;
   auto fetch = [&](uint32_t row0) {
-    const uint32_t row = row0 + r;
-    const bool live = row < rows;
-    const uint32_t i = live ? row / a.group : 0, h = live ? row % a.group : 0;
-    fetch_row<NG, NP, 1>(live, q_at<NG, NP>(a, b, gh, i, h), c, raw);
-    vis = live ? sees(a, len, count, i) : 0;
-    lse = row_lse(a, unit, live ? row : 0, c);
+    const size_t block = (size_t)unit * ((a.rows + 15) / 16) + row0 / 16;
+    static_for<0, NG>([&](auto G) {
+      static_for<0, 2>([&](auto S) {
+        static_for<0, NP>([&](auto P) { next.f[G][S][P] = a.operands[((block * NG + G) * 2 * NP + S * NP + P) * 64 + lane]; });
+      });
+    });
+    const RowFacts f = a.facts[block * 16 + r];
+    next.unit = f.unit, vis = f.sees;
+    static_for<0, NG>([&](auto G) { next.sum[G] = f.sum[G]; });
+    lse = row_lse(a, unit, row0 + r < rows ? row0 + r : 0, c);
   };
   uint32_t row0 = from / 16 * 16 + wave * 16;
   if (row0 < rows) fetch(row0);
   for (; row0 < rows; row0 += 16 * NW) {
-    QRow<NG, NP, 1> q;
-    make_row<NG, NP, 1>(a, raw, q);
+    const QRow<NG, NP, 1> q = next;
     const uint32_t end = vis;
     const float sub = lse;
     if (row0 + 16 * NW < rows) fetch(row0 + 16 * NW);
@@ -875,6 +912,7 @@ hipError_t launch_np(const Attn4& a, hipStream_t s) {
   }
   const uint32_t joins = a.split_slots ? units * a.rows : 0, slots = a.scores ? 64 * NW * 4 : 64;
   const uint32_t tiles = a.weight_out ? (a.max_len + slots - 1) / slots : 0;
+  if (a.operands) hipLaunchKernelGGL((cache4_operands_kernel<NG, NP>), dim3(units * ((a.rows + 15) / 16)), dim3(64), 0, s, a);
   if (joins || tiles) hipLaunchKernelGGL((cache4_finish_kernel<NG, NP>), dim3(joins + tiles * units), block, 0, s, a, joins, tiles);
   return hipGetLastError();
 }

@@ -8,6 +8,12 @@ constexpr size_t kScoreBytes = 256u << 20;
 // workgroups that run at once: two a CU up to head dim 128, where their rings are 74 KB of its 160, one above
 uint32_t slots_of(uint32_t dim) { return dim <= 128 ? 512 : 256; }
 
+// Weights of at most 16 rows come from the scores as the attention kernel had them, 4 bytes a row and slot, instead of from a
+// second pass over K with all its products; not where they would take more than kScoreBytes.
+bool stored_scores(const Cache4Attention& L, uint32_t rows) {
+  return rows <= 16 && (size_t)L.c.batch * L.c.kv_heads * rows * L.max_len * 4 <= kScoreBytes;
+}
+
 // rows a workgroup takes, and whether a sequence's tiles are shared out
 Attn4 plan_of(const Cache4Attention& L) {
   Attn4 a{};
@@ -28,7 +34,7 @@ Attn4 plan_of(const Cache4Attention& L) {
   return a;
 }
 
-// The scratch's parts, in order: part, ml, shares; lse; scores. Returns its bytes; sets the pointers when there is one.
+// The scratch's parts, in order: part, ml, shares; lse; scores or operands and facts. Returns its bytes; sets the pointers when there is one.
 size_t lay_out(const Cache4Attention& L, Attn4& a) {
   size_t n = 0;
   auto take = [&](size_t words) {
@@ -43,9 +49,13 @@ size_t lay_out(const Cache4Attention& L, Attn4& a) {
   } else if (L.weight_out) {
     a.lse = take(rows);
   }
-  // Weights of at most 16 rows come from the scores as the attention kernel had them, 4 bytes a row and slot, instead of from
-  // a second pass over K with all its products; not where they would take more than kScoreBytes.
-  if (L.weight_out && a.rows && a.rows <= 16 && rows * L.max_len * 4 <= kScoreBytes) a.scores = take(rows * L.max_len);
+  if (L.weight_out && a.rows && stored_scores(L, a.rows)) {
+    a.scores = take(rows * L.max_len);
+  } else if (L.weight_out && a.rows) {
+    const size_t blocks = (size_t)L.c.batch * L.c.kv_heads * ((a.rows + 15) / 16);
+    a.operands = (u32x4*)take(blocks * (L.c.dim / 64) * 2 * (L.dtype == F32 ? 2 : 1) * 64 * 4);
+    a.facts = (RowFacts*)take(blocks * 16 * sizeof(RowFacts) / 4);
+  }
   return n * 4;
 }
 
