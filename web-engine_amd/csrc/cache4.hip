@@ -189,15 +189,13 @@ __global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
   const size_t base = (size_t)unit * cap;
   const float* weight = a.weight + base;
   const int32_t* pos = a.pos + base;
-  const bool copy = a.weight_out != a.weight || a.pos_out != a.pos;
-  auto stay = [&](uint32_t s) {
-    if (a.weight_out != a.weight) a.weight_out[base + s] = weight[s];
-    if (a.pos_out != a.pos) a.pos_out[base + s] = pos[s];
-  };
   if (!g.late_lens && gh == 0 && t == 0) a.lens_out[b] = (int32_t)left;
+  // out of place, all that is below `left` is copied; the holes there are filled later, by the moves
+  if (a.weight_out != a.weight)
+    for (uint32_t s = t; s < left; s += EV_NT) a.weight_out[base + s] = weight[s];
+  if (a.pos_out != a.pos)
+    for (uint32_t s = t; s < left; s += EV_NT) a.pos_out[base + s] = pos[s];
   if (left == len) {
-    if (copy)
-      for (uint32_t s = t; s < len; s += EV_NT) stay(s);
     if (g.most > EV_FEW && t == 0) g.counts[unit] = 0;
     return;
   }
@@ -280,9 +278,6 @@ __global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
       for (uint32_t n = 0; n < EV_ONE_BY_ONE; n++) x |= gone[n] == s;
       return x;
     };
-    if (copy)
-      for (uint32_t s = t; s < left; s += EV_NT)
-        if (!is_gone(s)) stay(s);
     // the holes in order meet the slots from `left` on that stay
     uint32_t fill = left, hole = 0;
     for (uint32_t n = 0; n < go; n++) {
@@ -377,10 +372,10 @@ __global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
   };
   uint32_t holes = 0, fills = 0;
   each([&](uint32_t v, bool in, uint32_t k, bool p) {
-    const uint32_t s = from + v * 64 + lane;
+    const uint32_t s0 = from + v * 64;  // a piece lies below `left`, above it, or across
     const bool gone = gone_of(in, k, p);
-    holes += (uint32_t)__popcll(__ballot(gone && s < left));
-    fills += (uint32_t)__popcll(__ballot(in && !gone && s >= left));
+    if (s0 < left) holes += (uint32_t)__popcll(__ballot(gone && s0 + lane < left));
+    if (s0 + 64 > left) fills += (uint32_t)__popcll(__ballot(in && !gone && s0 + lane >= left));
   });
   __syncthreads();
   if (lane == 0) waves[0][wave] = holes, waves[1][wave] = fills;
@@ -394,13 +389,20 @@ __global__ void __launch_bounds__(EV_NT) cache4_select_kernel(EvictArgs g) {
   uint32_t* fill_list = g.most <= EV_FEW ? few[1] : hole_list + g.most;
   ties = first_tie;
   each([&](uint32_t v, bool in, uint32_t k, bool p) {
-    const uint32_t s = from + v * 64 + lane;
-    const bool gone = gone_of(in, k, p), hole = gone && s < left, fill = in && !gone && s >= left;
-    const uint64_t h = __ballot(hole), f = __ballot(fill);
-    if (hole) hole_list[holes + (uint32_t)__popcll(h & below)] = s;
-    if (fill) fill_list[fills + (uint32_t)__popcll(f & below)] = s;
-    holes += (uint32_t)__popcll(h), fills += (uint32_t)__popcll(f);
-    if (copy && in && !gone && s < left) stay(s);
+    const uint32_t s0 = from + v * 64, s = s0 + lane;
+    const bool gone = gone_of(in, k, p);
+    if (s0 < left) {
+      const bool hole = gone && s < left;
+      const uint64_t h = __ballot(hole);
+      if (hole) hole_list[holes + (uint32_t)__popcll(h & below)] = s;
+      holes += (uint32_t)__popcll(h);
+    }
+    if (s0 + 64 > left) {
+      const bool fill = in && !gone && s >= left;
+      const uint64_t f = __ballot(fill);
+      if (fill) fill_list[fills + (uint32_t)__popcll(f & below)] = s;
+      fills += (uint32_t)__popcll(f);
+    }
   });
   if (g.most <= EV_FEW) {
     __syncthreads();
