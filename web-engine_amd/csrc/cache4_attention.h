@@ -53,7 +53,7 @@ struct Attn4 {
   float* part;          // shared out: O [row block][slot][block_rows][dim], times 2^-m
   float* ml;            // and (m, l) [row block][slot][block_rows][2]
   uint32_t* shares;     // and each unit's first slot and its number of shares
-  float* lse;           // weights, not shared out: [unit][rows], log2 of a row's sum of 2^score
+  float* lse;           // weights, unless they come from shared-out scores: [unit][rows], log2 of a row's sum of 2^score
   float* scores;        // weights of at most 16 rows: [unit][rows][max_len], the scores in log2 units
   u32x4* operands;      // weights of more: the rows' operands [unit][16 rows][step and plane][lane]
   RowFacts* facts;      // and the rest of them [unit][row, up to a multiple of 16]
@@ -719,6 +719,7 @@ __device__ __forceinline__ void join_row(const Attn4& a, uint32_t ur) {
   }
   __syncthreads();
   if (side) return;
+  if (a.lse && threadIdx.x == 0) a.lse[ur] = top + __builtin_amdgcn_logf(l);
 #pragma unroll
   for (int x = 1; x < SIDE; x++) v += sums[x][d];
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
@@ -786,12 +787,13 @@ __device__ __forceinline__ void receive_scores(const Attn4& a, uint32_t unit, ui
     if (k + e < len) a.weight_out[slot + e] = (a.weight ? a.weight[slot + e] : 0.0f) + sum[e];
 }
 
-// The operands of all rows for `receive`, a wave per 16 of a unit. A launch of its own: written by the attention kernel, they
-// cost its loop more in registers (2048 queries over 8192 slots 380 -> 405 us) than the launch takes.
+// The operands of 16 rows for `receive`, by a wave. (Written by the attention kernel, they cost its loop more in registers, 2048
+// queries over 8192 slots 380 -> 405 us, than this takes.)
 template <int NG, int NP>
-__global__ void __launch_bounds__(64) cache4_operands_kernel(Attn4 a) {
-  const uint32_t blocks = (a.rows + 15) / 16, unit = blockIdx.x / blocks, row0 = blockIdx.x % blocks * 16;
-  const int lane = threadIdx.x, r = lane & 15, c = lane >> 4;
+__device__ __forceinline__ void keep_operands(const Attn4& a, uint32_t block) {
+  const uint32_t blocks = (a.rows + 15) / 16, unit = block / blocks, row0 = block % blocks * 16;
+  if (unit >= a.batch * a.kv_heads) return;
+  const int lane = threadIdx.x & 63, r = lane & 15, c = lane >> 4;
   uint32_t len, count;
   unit_of(a, unit, len, count);
   const uint32_t row = row0 + r, rows = count * a.group;
@@ -804,14 +806,14 @@ __global__ void __launch_bounds__(64) cache4_operands_kernel(Attn4 a) {
   make_row<NG, NP, 1>(a, raw, q);
   static_for<0, NG>([&](auto G) {
     static_for<0, 2>([&](auto S) {
-      static_for<0, NP>([&](auto P) { a.operands[(((size_t)blockIdx.x * NG + G) * 2 * NP + S * NP + P) * 64 + lane] = q.f[G][S][P]; });
+      static_for<0, NP>([&](auto P) { a.operands[(((size_t)block * NG + G) * 2 * NP + S * NP + P) * 64 + lane] = q.f[G][S][P]; });
     });
   });
   if (c) return;
   RowFacts f{};
   f.unit = q.unit, f.sees = live ? sees(a, len, count, i) : 0;
   static_for<0, NG>([&](auto G) { f.sum[G] = q.sum[G]; });
-  a.facts[(size_t)blockIdx.x * 16 + r] = f;
+  a.facts[(size_t)block * 16 + r] = f;
 }
 
 // The attention each slot received, from the cache: a workgroup takes 64 slots and its waves the query rows, every NW-th
@@ -855,7 +857,7 @@ __device__ __forceinline__ void receive(const Attn4& a, uint32_t unit, uint32_t 
     const RowFacts f = a.facts[block * 16 + r];
     next.unit = f.unit, vis = f.sees;
     static_for<0, NG>([&](auto G) { next.sum[G] = f.sum[G]; });
-    lse = row_lse(a, unit, row0 + r < rows ? row0 + r : 0, c);
+    lse = a.lse[(size_t)unit * a.rows + (row0 + r < rows ? row0 + r : 0)];
   };
   uint32_t row0 = from / 16 * 16 + wave * 16;
   if (row0 < rows) fetch(row0);
@@ -887,17 +889,18 @@ __device__ __forceinline__ void receive(const Attn4& a, uint32_t unit, uint32_t 
   a.weight_out[slot + threadIdx.x] = (a.weight ? a.weight[slot + threadIdx.x] : 0.0f) + mine;
 }
 
-// What follows the attention kernel, in one launch: first a workgroup per row whose shares are to be joined, then those of a
-// unit's slots that receive weight.
+// What follows the attention kernel: first a workgroup per row whose shares are to be joined, then those of a unit's slots that
+// receive weight from stored scores, or of the rows whose operands the slots go by.
 template <int NG, int NP>
 __global__ void __launch_bounds__(64 * NW) cache4_finish_kernel(Attn4 a, uint32_t joins, uint32_t tile_blocks) {
-  if (blockIdx.x < joins) {
-    join_row<NG>(a, blockIdx.x);
-  } else {
-    const uint32_t x = blockIdx.x - joins;
-    if (a.scores) receive_scores(a, x / tile_blocks, x % tile_blocks);
-    else receive<NG, NP>(a, x / tile_blocks, x % tile_blocks);
-  }
+  const uint32_t x = blockIdx.x - joins;
+  if (blockIdx.x < joins) join_row<NG>(a, blockIdx.x);
+  else if (a.scores) receive_scores(a, x / tile_blocks, x % tile_blocks);
+  else keep_operands<NG, NP>(a, x * NW + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
+}
+template <int NG, int NP>
+__global__ void __launch_bounds__(64 * NW) cache4_receive_kernel(Attn4 a, uint32_t tiles) {
+  receive<NG, NP>(a, blockIdx.x / tiles, blockIdx.x % tiles);
 }
 
 template <int NG, int NP>
@@ -910,10 +913,13 @@ hipError_t launch_np(const Attn4& a, hipStream_t s) {
     else if (a.rt == 1) hipLaunchKernelGGL((cache4_attention_kernel<NG, 1, NP, 1>), grid, block, 0, s, a);
     else if constexpr (most_rows(NG) == 2) hipLaunchKernelGGL((cache4_attention_kernel<NG, 2, NP, 1>), grid, block, 0, s, a);
   }
-  const uint32_t joins = a.split_slots ? units * a.rows : 0, slots = a.scores ? 64 * NW * 4 : 64;
-  const uint32_t tiles = a.weight_out ? (a.max_len + slots - 1) / slots : 0;
-  if (a.operands) hipLaunchKernelGGL((cache4_operands_kernel<NG, NP>), dim3(units * ((a.rows + 15) / 16)), dim3(64), 0, s, a);
-  if (joins || tiles) hipLaunchKernelGGL((cache4_finish_kernel<NG, NP>), dim3(joins + tiles * units), block, 0, s, a, joins, tiles);
+  const uint32_t joins = a.split_slots ? units * a.rows : 0, per = 64 * NW * 4, blocks = (a.max_len + per - 1) / per;
+  const uint32_t more = a.scores ? units * blocks : a.operands ? (units * ((a.rows + 15) / 16) + NW - 1) / NW : 0;
+  if (joins || more) hipLaunchKernelGGL((cache4_finish_kernel<NG, NP>), dim3(joins + more), block, 0, s, a, joins, blocks);
+  if (a.weight_out && !a.scores) {
+    const uint32_t tiles = (a.max_len + 63) / 64;
+    hipLaunchKernelGGL((cache4_receive_kernel<NG, NP>), dim3(units * tiles), block, 0, s, a, tiles);
+  }
   return hipGetLastError();
 }
 

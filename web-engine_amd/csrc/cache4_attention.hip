@@ -23,11 +23,12 @@ Attn4 plan_of(const Cache4Attention& L) {
   a.block_rows = 16 * a.rt / a.pk;
   a.row_blocks = (a.rows + a.block_rows - 1) / a.block_rows;
   const uint64_t units = (uint64_t)L.c.batch * L.c.kv_heads, blocks = units * a.row_blocks;
-  // Shared out where the units alone leave half of the chip idle and a sequence may have at least eight tiles for each of a
-  // workgroup's waves: fewer take less than the second launch and the sharing do (72 units of 17 tiles, f32: 9.8 us by a
-  // workgroup each, 13.2 us in three shares; 64 units of up to 64 tiles with weights: 25.9 us, 23.0 in shares)
+  // Shared out where the units alone leave half of the chip idle and a sequence may have so many tiles that a workgroup takes
+  // longer over them than the second launch and the sharing do: 32 of one block of 16 rows and 128 values, fewer of more (72
+  // units of 17 tiles, f32 of 64 values: 9.8 us by a workgroup each, 13.2 us in three shares; 64 units of up to 64 tiles with
+  // weights: 25.9 us, 23.0 in shares; 2 units of 18 tiles of 256 values: 20.7 us, 17.0 in shares)
   const uint32_t slots = slots_of(L.c.dim);
-  if (a.rows && blocks <= slots / 2 && L.c.batch <= kMostShared && (L.max_len + 63) / 64 >= 8 * NW) {
+  if (a.rows && blocks <= slots / 2 && L.c.batch <= kMostShared && (uint64_t)((L.max_len + 63) / 64) * a.rt * (L.c.dim / 64) >= 64) {
     a.split_slots = slots / a.row_blocks;
     a.split_slots = a.split_slots > units ? a.split_slots : (uint32_t)units;
   }
@@ -46,9 +47,8 @@ size_t lay_out(const Cache4Attention& L, Attn4& a) {
   if (a.split_slots) {
     const size_t shares = (size_t)a.row_blocks * a.split_slots * a.block_rows;
     a.part = take(shares * L.c.dim), a.ml = take(shares * 2), a.shares = (uint32_t*)take((size_t)L.c.batch * L.c.kv_heads * 2);
-  } else if (L.weight_out) {
-    a.lse = take(rows);
   }
+  if (L.weight_out && !(a.split_slots && stored_scores(L, a.rows))) a.lse = take(rows);
   if (L.weight_out && a.rows && stored_scores(L, a.rows)) {
     a.scores = take(rows * L.max_len);
   } else if (L.weight_out && a.rows) {
