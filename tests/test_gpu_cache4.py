@@ -559,6 +559,30 @@ def test_captured_decode_step_replays(scope, stream):
         g.join()
 
 
+def test_rows_of_a_fused_projection(scope):
+    """q, k and v as columns of one QKV row, read by stride, with the projection's own norm and rotation before: the same
+    bytes as from packed copies."""
+    g, rng = scope, np.random.default_rng(41)
+    batch, heads, kv, d, hidden = 3, 4, 2, 128, 256
+    n = (heads + 2 * kv) * d
+    x = g.buffer(C.store(rng.standard_normal((batch, hidden)), we.BF16))
+    w = g.buffer(C.store(rng.standard_normal((n, hidden)) / 16, we.BF16))
+    ones, angle = g.buffer(np.zeros(d, np.float32)), rng.uniform(0, 6, (batch, d // 2)).astype(np.float32)
+    qkv = g.buffer(batch * n * 2)
+    g.matmul_qk_norm_rope(we.matmul_params(batch, n, hidden, 1.0, graph=g), we.BF16, x, we.BF16, w, we.BF16, qkv, heads, kv, 1e-6,
+                          1.0, ones, ones, 0, g.buffer(np.cos(angle)), g.buffer(np.sin(angle)))
+    a = g.read(qkv, dtype=np.uint16).reshape(batch, n)
+    parts = [g.buffer(np.ascontiguousarray(p)) for p in np.split(a, [heads * d, (heads + kv) * d], 1)]
+    got = []
+    for q, k, v, st in ((qkv, qkv.ptr + heads * d * 2, qkv.ptr + (heads + kv) * d * 2, n), (*parts, 0)):
+        c = we.Cache4(g, batch, kv, d, 64)
+        for _ in range(2):
+            c.append(k, v, 1, we.BF16, k_stride=st, v_stride=st)
+        y = c.attention(q, 1, heads, we.BF16, q_stride=st, track=True)
+        got.append([g.read(b) for b in (y, c.data, c.weight)])
+    assert all(np.array_equal(p, q) for p, q in zip(*got)) and got[0][0].any()
+
+
 def test_two_streams_at_once(scope):
     """Calls on both compute streams, each with its own scratch, queued without a wait between them."""
     g, rng = scope, np.random.default_rng(40)
