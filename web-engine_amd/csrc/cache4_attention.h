@@ -644,40 +644,30 @@ __global__ void __launch_bounds__(64 * NW, NG <= 2 ? 2 : 1) cache4_attention_ker
   while (t < t1) step(std::true_type{});
 
   // join the waves, and a row's PK columns: the largest maximum, all sums brought to it, their total
-  float* ml = (float*)lds;                         // [wave][16][2]
-  float* joined = ml + NW * 16 * 2;                // [wave][16][ROW]
+  float* ml = (float*)lds;           // [wave][16][2]
+  float* joined = ml + NW * 16 * 2;  // [wave][16][ROW]
   static_for<0, RT>([&](auto I) {
     const float l = row_sum(le[I] + 16.0f * lo[I]);
     __syncthreads();
     if (c == 0) ml[(wave * 16 + r) * 2] = m[I], ml[(wave * 16 + r) * 2 + 1] = l;
-    __syncthreads();
-    float top = kNone, total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < NW * PK; w++) top = fmaxf(top, ml[(w * C::kRows + r % C::kRows) * 2]);
-    const float f = __builtin_amdgcn_exp2f(m[I] - top);
-#pragma unroll
-    for (int w = 0; w < NW * PK; w++) {
-      const int x = (w * C::kRows + r % C::kRows) * 2;
-      total += ml[x + 1] * __builtin_amdgcn_exp2f(ml[x] - top);
-    }
     static_for<0, NG>([&](auto G) {
       const float mn = row_sum(me[I][G] + 16.0f * mo[I][G]);
-      static_for<0, 4>([&](auto D) {
-        f32x4 v;
-        static_for<0, 4>([&](auto E) { v[E()] = f * (o[I][4 * G + D][E()] + mn); });
-        *(f32x4*)(joined + (wave * 16 + r) * ROW + (4 * G + D) * 16 + 4 * c) = v;
-      });
+      static_for<0, 4>([&](auto D) { *(f32x4*)(joined + (wave * 16 + r) * ROW + (4 * G + D) * 16 + 4 * c) = o[I][4 * G + D] + mn; });
     });
-    __syncthreads();
-    if (wave == 0 && c == 0 && r < C::kRows) ml[r * 2] = top, ml[r * 2 + 1] = total;  // read by all below
     __syncthreads();
     for (uint32_t x = threadIdx.x; x < C::kRows * DIM / 4; x += 64 * NW) {
       const uint32_t rr = x / (DIM / 4), d = x % (DIM / 4) * 4, row = row0 + 16 * I + rr;
       if (row >= rows) continue;
+      float mm = kNone, ll = 0.0f;
+#pragma unroll
+      for (int w = 0; w < NW * PK; w++) mm = fmaxf(mm, ml[(w * C::kRows + rr) * 2]);
       f32x4 v = {};
 #pragma unroll
-      for (int w = 0; w < NW * PK; w++) v += *(const f32x4*)(joined + (w * C::kRows + rr) * ROW + d);
-      const float mm = ml[rr * 2], ll = ml[rr * 2 + 1];
+      for (int w = 0; w < NW * PK; w++) {
+        const float f = __builtin_amdgcn_exp2f(ml[(w * C::kRows + rr) * 2] - mm);
+        ll = __builtin_fmaf(f, ml[(w * C::kRows + rr) * 2 + 1], ll);
+        v += f * *(const f32x4*)(joined + (w * C::kRows + rr) * ROW + d);
+      }
       if (a.split_slots) {
         const size_t at = ((size_t)rb * a.split_slots + slot) * ROWS + 16 * I + rr;
         *(f32x4*)(a.part + at * DIM + d) = v;
@@ -692,8 +682,8 @@ __global__ void __launch_bounds__(64 * NW, NG <= 2 ? 2 : 1) cache4_attention_ker
   });
 }
 
-// The shares of a row joined by one workgroup (bound by latency: 128 rows of 16 shares 4.5 us): DIM / 4 threads a share, several shares at once, brought to the largest
-// maximum and summed in a fixed order.
+// The shares of a row joined by one workgroup (bound by latency: 128 rows of 16 shares 4.5 us): DIM / 4 threads a share,
+// several shares at once, brought to the largest maximum and summed in a fixed order.
 template <int NG>
 __device__ __forceinline__ void join_row(const Attn4& a, uint32_t ur) {
   constexpr int DIM = 64 * NG, LANES = DIM / 4, SIDE = 64 * NW / LANES;

@@ -1523,10 +1523,10 @@ int check_operands(we_ctx* ctx, const Operand* ops, size_t n) {
       if (const int rc = check_span(ctx, ops[i].p, ops[i].bytes, ops[i].name)) return rc;
     }
   for (size_t i = 0; i < n; i++) {
-    if (!ops[i].p || !ops[i].written) continue;
+    if (!ops[i].p || !ops[i].bytes || !ops[i].written) continue;
     const uintptr_t a = (uintptr_t)ops[i].p;
     for (size_t j = 0; j < n; j++) {
-      if (j == i || !ops[j].p || (ops[j].written && j < i)) continue;
+      if (j == i || !ops[j].p || !ops[j].bytes || (ops[j].written && j < i)) continue;
       if (!ops[j].written && ops[j].p == ops[i].same) continue;
       const uintptr_t b = (uintptr_t)ops[j].p;
       if (a < b + ops[j].bytes && b < a + ops[i].bytes)
