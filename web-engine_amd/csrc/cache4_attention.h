@@ -21,7 +21,7 @@
 // Bounds and figures (MI355X; head dim 128). A decode step reads 4.5 bits a value, so it is bound by HBM once it is long: 4
 // sequences of up to 65521 slots, 32 / 8 heads, f16: 245 MB in 47 us with the join, 5.2 TB/s (a streaming read reaches 6.8),
 // 41 us of them in the attention kernel, about 4 before the first tile is there. A short one is bound by latency: 131 slots
-// 5.5 us, of which a wave's one tile takes 1.7 us and the join of the waves 1.1. A prompt is bound by the vector unit, which
+// 5.5 us, of which a wave's one tile takes 1.7 us and the join of the waves 0.9. A prompt is bound by the vector unit, which
 // is busy 90% of the time (the MFMA 28%): 2048 queries over 8192 slots, 32 / 8 heads, f16: 379 us, 0.63 PFLOP/s.
 #pragma once
 #include "common.h"

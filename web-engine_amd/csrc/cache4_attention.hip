@@ -6,6 +6,7 @@ namespace {
 
 constexpr size_t kScoreBytes = 256u << 20;
 // workgroups that run at once: two a CU up to head dim 128, where their rings are 74 KB of its 160, one above
+// (head dim 128, 16 sequences up to 4093 slots / 4 up to 65521: 512 workgroups 21.7 / 46.6 us, 768 26.5 / 51.7, 1024 30.3 / 49.9)
 uint32_t slots_of(uint32_t dim) { return dim <= 128 ? 512 : 256; }
 
 // Weights of at most 16 rows come from the scores as the attention kernel had them, 4 bytes a row and slot, instead of from a
